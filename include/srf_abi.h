@@ -48,6 +48,9 @@ enum { SRF_SAMPLING_ORIGINAL = 0, SRF_SAMPLING_DISPARITY = 1, SRF_SAMPLING_LOG =
 enum { SRF_GRID_WARPED_EXP = 0, SRF_GRID_WARPED_RECIPROCAL = 1, SRF_GRID_METRIC_EXP = 2,
        SRF_GRID_METRIC_RECIPROCAL = 3 };
 
+/* Value types of the layer operators (srf_grouped_matmul and its neighbours). No counterpart in the reference. */
+enum { SRF_TYPE_F16 = 0, SRF_TYPE_BF16 = 1, SRF_TYPE_F32 = 2, SRF_TYPE_E4M3 = 3 };
+
 /* Which field answers (r,g,b,sigma) for a sample. */
 enum { SRF_FIELD_NETWORK = 0,     /* hash grid + SH + two MLPs (internal/network/ngp_network.h) */
        SRF_FIELD_BLOBS = 1 };     /* closed-form Gaussian blobs, fp32: a seed-generated stand-in scene */
@@ -314,6 +317,68 @@ srf_status srf_volume_rendering_loss(srf_ctx* ctx, const srf_loss_params_t* para
                                      uint32_t* d_n_compacted_counter, uint16_t* d_dloss_doutput, float* d_loss_output,
                                      float* d_reg_distortion, void* stream);
 
+/* ---- layers of fields cut into regions ------------------------------------------------------
+   No counterpart in the reference, which has one network (internal/network/ngp_network.h).  A scene too large for one
+   network is cut into regions with a network each; the samples of a frame or batch, sorted by region, then go through
+   each layer as one matrix product per region.  Sample-major arrays hold all samples, region after region: group g owns
+   rows d_offsets[g] .. d_offsets[g+1], the layout srf_sample_offsets makes of per-region counts.  Rows in front of
+   d_offsets[0] and behind d_offsets[n_groups] are neither used nor written.
+
+   Rules of all these calls:
+     - matrices are row-major [n_out][n_in], as the network's own layers;
+     - row strides and group_stride are in elements (0: no gap); base addresses and strides are multiples of 16 bytes (pad
+       odd widths: columns between the width and the stride are neither read nor written);
+     - an output array overlaps no input array;
+     - d_offsets is read on the device, so the counts of a stage before need not come to the host.  Offsets that run
+       backwards or point behind n_rows are cut to the buffer and reported by srf_check_errors as SRF_ERR_ARG; the
+       call's output is then meaningless (n_rows = 0 launches no product and reports nothing).  d_offsets NULL: one
+       group of all n_rows rows (n_groups = 1);
+     - products are summed in fp32 and rounded once to out_type; no call allocates, synchronises or keeps state, so all
+       of them can be captured, and calls on different streams may overlap. */
+typedef struct srf_grouped_t {
+    uint32_t struct_size;        /* sizeof(srf_grouped_t), checked */
+    uint32_t n_groups;           /* 1 .. 4096 */
+    uint64_t n_rows;             /* rows of the sample-major arrays (a capacity: the offsets say which are used), < 2^31 */
+    uint32_t n_in, n_out;        /* layer widths, 1 .. 65536 */
+    int32_t  type;               /* of the operands: SRF_TYPE_F16, SRF_TYPE_BF16; SRF_TYPE_E4M3 for srf_grouped_matmul_fp8 */
+    int32_t  out_type;           /* of the result: `type` or SRF_TYPE_F32; F16, BF16 or F32 for srf_grouped_matmul_fp8 */
+    int32_t  activation;         /* SRF_ACT_NONE or SRF_ACT_RELU on the result of a layer; SRF_ACT_NONE for gradients */
+    uint32_t reserved;           /* 0 */
+    uint64_t ld_x, ld_w, ld_y;   /* row strides of n_in-wide samples, of matrices, of n_out-wide samples; 0: the width */
+    uint64_t group_stride;       /* between two groups' matrices; 0: n_out * ld_w */
+} srf_grouped_t;
+
+/* y[r] = act(W[g] x[r]): d_x [n_rows][n_in], d_w [n_groups][n_out][n_in], d_y [n_rows][n_out] of out_type. */
+srf_status srf_grouped_matmul(srf_ctx* ctx, const srf_grouped_t* p, const uint64_t* d_offsets, const void* d_x, const void* d_w,
+                              void* d_y, void* stream);
+/* dx[r] = W[g]^T dy[r]: d_dy [n_rows][n_out], d_dx [n_rows][n_in] of out_type.  d_gate (may be NULL) [n_rows][n_in] of
+   `type`, strided by ld_x: the layer's input where that came from a ReLU; dx is 0 where the gate is not > 0. */
+srf_status srf_grouped_input_grad(srf_ctx* ctx, const srf_grouped_t* p, const uint64_t* d_offsets, const void* d_dy,
+                                  const void* d_w, const void* d_gate, void* d_dx, void* stream);
+/* dW[g] = sum over the group's samples of dy[r] x[r]^T, every entry set (0 for a group without samples): d_dw
+   [n_groups][n_out][n_in] of out_type, strided by ld_w and group_stride.  The sum's order is fixed by the sizes and the
+   device, so the result is the same on every run.  n_rows <= 2^26.  d_workspace: srf_grouped_weight_grad_workspace bytes
+   (16-byte aligned), free again when the call's work is done; calls that may overlap need one each. */
+srf_status srf_grouped_weight_grad(srf_ctx* ctx, const srf_grouped_t* p, const uint64_t* d_offsets, const void* d_dy,
+                                   const void* d_x, void* d_dw, void* d_workspace, size_t workspace_bytes, void* stream);
+srf_status srf_grouped_weight_grad_workspace(srf_ctx* ctx, const srf_grouped_t* p, size_t* bytes);
+
+/* srf_grouped_matmul on 8-bit values: y[r] = act(sum over blocks b of 128 inputs of
+   d_x_scales[b][r] * d_w_scales[g][n/128][b] * (W[g] x[r])_b), with d_x_scales float[ceil(n_in/128)][n_rows] and
+   d_w_scales float[n_groups][ceil(n_out/128)][ceil(n_in/128)] as the two calls below write them. */
+srf_status srf_grouped_matmul_fp8(srf_ctx* ctx, const srf_grouped_t* p, const uint64_t* d_offsets, const void* d_x,
+                                  const float* d_x_scales, const void* d_w, const float* d_w_scales, void* d_y, void* stream);
+/* Samples to e4m3 with one scale per row and 128 columns: s = max |v| / 448 over the block's finite values (1 if that is 0,
+   at least 2^-126), q = the e4m3 value nearest to v / s, ties to even; infinities and NaNs become NaN.  d_in [n_rows][n_cols] of `type` (F16, BF16), d_out
+   e4m3 [n_rows][n_cols], d_scales float[ceil(n_cols/128)][n_rows].  d_n_rows_used (may be NULL: all): device counter,
+   rows from it on are left as they are (d_offsets + n_groups serves). */
+srf_status srf_quantize_rows(srf_ctx* ctx, int type, uint64_t n_rows, const uint64_t* d_n_rows_used, uint32_t n_cols,
+                             const void* d_in, uint64_t ld_in, void* d_out, uint64_t ld_out, float* d_scales, void* stream);
+/* Matrices to e4m3 with one scale per 128 x 128 block: d_in [n_matrices][n_rows][n_cols], d_out likewise, d_scales
+   float[n_matrices][ceil(n_rows/128)][ceil(n_cols/128)].  Strides of matrices: n_rows * ld. */
+srf_status srf_quantize_weights(srf_ctx* ctx, int type, uint32_t n_matrices, uint32_t n_rows, uint32_t n_cols, const void* d_in,
+                                uint64_t ld_in, void* d_out, uint64_t ld_out, float* d_scales, void* stream);
+
 /* ---- whole frames ------------------------------------------------------------------------ */
 
 /* Testbed::render_frame (internal/testbed.cu:479-606) for one sample-per-pixel pass of one
@@ -393,7 +458,7 @@ srf_status srf_dump_samples(srf_ctx* ctx, const srf_view_t* view, uint64_t ray_f
 
 /* Device-side error word of the context (the reference has none: its kernels cannot time out).  Bits: 1 = a
    ray hit the march loop's iteration bound, 2 = a wait on the tensor-core commit barrier expired, 4 = the
-   sample pool ran out of chunks.  Frames enqueued without `stats` do not synchronise and therefore cannot
+   sample pool ran out of chunks, 16 = a layer call met offsets outside its buffers (reported as SRF_ERR_ARG).  Frames enqueued without `stats` do not synchronise and therefore cannot
    report; the word stays set across frames until one of srf_render, srf_dump_samples, a frame with `stats`
    or this call has returned it as SRF_ERR_TIMEOUT / SRF_ERR_CAPACITY, which also clears it.  Synchronises
    `stream`.  `flags` (may be NULL) receives the raw word. */

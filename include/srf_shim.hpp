@@ -93,6 +93,35 @@ private:
     Context& m;
 };
 
+// The layers of networks per region (no counterpart in the reference): see srf_grouped_t.
+class GroupedLayer {
+public:
+    GroupedLayer(Context& c, const srf_grouped_t& p) : m(c), m_p(p) {}
+    srf_grouped_t& params() { return m_p; }
+    void forward(const uint64_t* d_offsets, const void* d_x, const void* d_w, void* d_y, void* stream) {
+        check(srf_grouped_matmul(m.get(), &m_p, d_offsets, d_x, d_w, d_y, stream), m.get());
+    }
+    void forward_fp8(const uint64_t* d_offsets, const void* d_x, const float* d_x_scales, const void* d_w, const float* d_w_scales,
+                     void* d_y, void* stream) {
+        check(srf_grouped_matmul_fp8(m.get(), &m_p, d_offsets, d_x, d_x_scales, d_w, d_w_scales, d_y, stream), m.get());
+    }
+    void input_grad(const uint64_t* d_offsets, const void* d_dy, const void* d_w, const void* d_gate, void* d_dx, void* stream) {
+        check(srf_grouped_input_grad(m.get(), &m_p, d_offsets, d_dy, d_w, d_gate, d_dx, stream), m.get());
+    }
+    size_t weight_grad_workspace() const {
+        size_t n = 0;
+        check(srf_grouped_weight_grad_workspace(m.get(), &m_p, &n), m.get());
+        return n;
+    }
+    void weight_grad(const uint64_t* d_offsets, const void* d_dy, const void* d_x, void* d_dw, void* d_workspace,
+                     size_t workspace_bytes, void* stream) {
+        check(srf_grouped_weight_grad(m.get(), &m_p, d_offsets, d_dy, d_x, d_dw, d_workspace, workspace_bytes, stream), m.get());
+    }
+private:
+    Context& m;
+    srf_grouped_t m_p;
+};
+
 // internal/render/ray_marcher.h:13-81
 class RayMarcher {
 public:

@@ -25,6 +25,7 @@ WARP_NGP, WARP_MIPNERF360, WARP_DONERF, WARP_SIGMOID, WARP_ERP, WARP_SINUSOIDAL 
 SAMPLING_ORIGINAL, SAMPLING_DISPARITY, SAMPLING_LOG = range(3)
 GRID_WARPED_EXP, GRID_WARPED_RECIPROCAL, GRID_METRIC_EXP, GRID_METRIC_RECIPROCAL = range(4)
 FIELD_NETWORK, FIELD_BLOBS = range(2)
+TYPE_F16, TYPE_BF16, TYPE_F32, TYPE_E4M3 = range(4)   # value types of the layer operators
 
 
 class Config(C.Structure):
@@ -77,6 +78,14 @@ class LossParams(C.Structure):
         ("regularization_type", C.c_int32), ("background_color", C.c_float * 3), ("color_space", C.c_int32),
         ("train_with_random_bg_color", C.c_int32), ("rng_state", C.c_uint64), ("rng_inc", C.c_uint64),
         ("padded_output_width", C.c_uint32),
+    ]
+
+
+class Grouped(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("n_groups", C.c_uint32), ("n_rows", C.c_uint64), ("n_in", C.c_uint32), ("n_out", C.c_uint32),
+        ("type", C.c_int32), ("out_type", C.c_int32), ("activation", C.c_int32), ("reserved", C.c_uint32),
+        ("ld_x", C.c_uint64), ("ld_w", C.c_uint64), ("ld_y", C.c_uint64), ("group_stride", C.c_uint64),
     ]
 
 
@@ -158,6 +167,17 @@ def make_view(camera, width, height, relative_focal_length, principal_point=(0.5
     return v
 
 
+def make_grouped(n_groups, n_rows, n_in, n_out, type=TYPE_F16, out_type=None, activation=ACT_NONE, ld_x=0, ld_w=0, ld_y=0,
+                 group_stride=0) -> Grouped:
+    """srf_grouped_t: strides in elements, 0 for arrays without gaps; out_type defaults to `type`."""
+    g = Grouped()
+    g.struct_size = C.sizeof(Grouped)
+    g.n_groups, g.n_rows, g.n_in, g.n_out = n_groups, n_rows, n_in, n_out
+    g.type, g.out_type, g.activation = type, type if out_type is None else out_type, activation
+    g.ld_x, g.ld_w, g.ld_y, g.group_stride = ld_x, ld_w, ld_y, group_stride
+    return g
+
+
 _P = C.POINTER
 _vp = C.c_void_p
 _ctx = C.c_void_p
@@ -207,6 +227,13 @@ SYMBOLS = {
                                            C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "srf_volume_rendering_loss": (C.c_int, [_ctx, _P(LossParams), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "srf_sample_offsets_static": (C.c_int, [C.c_int, _vp, C.c_uint64, _vp, _vp, C.c_char_p, C.c_size_t]),
+    "srf_grouped_matmul": (C.c_int, [_ctx, _P(Grouped), _vp, _vp, _vp, _vp, _vp]),
+    "srf_grouped_input_grad": (C.c_int, [_ctx, _P(Grouped), _vp, _vp, _vp, _vp, _vp, _vp]),
+    "srf_grouped_weight_grad": (C.c_int, [_ctx, _P(Grouped), _vp, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
+    "srf_grouped_weight_grad_workspace": (C.c_int, [_ctx, _P(Grouped), _P(C.c_size_t)]),
+    "srf_grouped_matmul_fp8": (C.c_int, [_ctx, _P(Grouped), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "srf_quantize_rows": (C.c_int, [_ctx, C.c_int, C.c_uint64, _vp, C.c_uint32, _vp, C.c_uint64, _vp, C.c_uint64, _vp, _vp]),
+    "srf_quantize_weights": (C.c_int, [_ctx, C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, _vp, C.c_uint64, _vp, C.c_uint64, _vp, _vp]),
     "srf_eval_math": (C.c_int, [C.c_int, C.c_int, _vp, _vp, _vp, C.c_size_t]),
 }
 

@@ -23,6 +23,8 @@
 #include <nvtx3/nvToolsExt.h>
 
 #include "srf_kernels.cuh"
+#include "srf_layer_args.h"
+#include "srf_layers.cuh"
 
 using namespace srf;
 
@@ -361,6 +363,7 @@ srf_status report_error_flags(srf_ctx* ctx, uint32_t flags, cudaStream_t s) {
     if (flags & 2u) return fail(ctx, SRF_ERR_TIMEOUT, "a wait on the tensor-core commit barrier expired");
     if (flags & 4u) return fail(ctx, SRF_ERR_CAPACITY, "the sample pool ran out of chunks");
     if (flags & 8u) return fail(ctx, SRF_ERR_STATE, "the fused grid refresh met a masked cell (the grid was changed behind the context)");
+    if (flags & 16u) return fail(ctx, SRF_ERR_ARG, "group offsets run backwards or point behind n_rows");
     return fail(ctx, SRF_ERR_CUDA, "unknown device error flag");
 }
 
@@ -982,6 +985,94 @@ srf_status srf_network_density(srf_ctx* ctx, const float* d_positions, uint64_t 
     launch_field_density(ctx->net, ctx->table, ctx->w_density, d_positions, 3, n, (__half*)d_out, (cudaStream_t)stream);
     SRF_CK(ctx, cudaGetLastError());
     return SRF_OK;
+}
+
+// ---- layers of fields cut into regions ------------------------------------------------------------
+
+}  // extern "C"
+
+namespace {
+
+srf_status launched(srf_ctx* ctx, const char* why) {
+    if (why) return fail(ctx, SRF_ERR_CUDA, why);
+    SRF_CK(ctx, cudaGetLastError());
+    return SRF_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+srf_status srf_grouped_matmul(srf_ctx* ctx, const srf_grouped_t* in, const uint64_t* d_offsets, const void* d_x, const void* d_w,
+                              void* d_y, void* stream) {
+    if (!ctx) return SRF_ERR_ARG;
+    srf_grouped_t p;
+    const std::string why = refuse_matmul(in, d_offsets, d_x, d_w, d_y, &p);
+    if (!why.empty()) return fail(ctx, SRF_ERR_ARG, why);
+    DeviceGuard guard(ctx->device);
+    return launched(ctx, launch_grouped_matmul(p, d_offsets, d_x, d_w, d_y, &ctx->d_counters->error_flags, (cudaStream_t)stream));
+}
+
+srf_status srf_grouped_input_grad(srf_ctx* ctx, const srf_grouped_t* in, const uint64_t* d_offsets, const void* d_dy, const void* d_w,
+                                  const void* d_gate, void* d_dx, void* stream) {
+    if (!ctx) return SRF_ERR_ARG;
+    srf_grouped_t p;
+    const std::string why = refuse_input_grad(in, d_offsets, d_dy, d_w, d_gate, d_dx, &p);
+    if (!why.empty()) return fail(ctx, SRF_ERR_ARG, why);
+    DeviceGuard guard(ctx->device);
+    return launched(ctx, launch_grouped_input_grad(p, d_offsets, d_dy, d_w, d_gate, d_dx, &ctx->d_counters->error_flags, (cudaStream_t)stream));
+}
+
+srf_status srf_grouped_weight_grad_workspace(srf_ctx* ctx, const srf_grouped_t* in, size_t* bytes) {
+    if (!ctx || !bytes) return SRF_ERR_ARG;
+    srf_grouped_t p;
+    const std::string why = refuse_weight_grad_shape(in, &p);
+    if (!why.empty()) return fail(ctx, SRF_ERR_ARG, why);
+    DeviceGuard guard(ctx->device);
+    *bytes = grouped_weight_grad_workspace(p, sm_count());
+    return SRF_OK;
+}
+
+srf_status srf_grouped_weight_grad(srf_ctx* ctx, const srf_grouped_t* in, const uint64_t* d_offsets, const void* d_dy, const void* d_x,
+                                   void* d_dw, void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (!ctx) return SRF_ERR_ARG;
+    srf_grouped_t p;
+    const std::string why = refuse_weight_grad(in, d_offsets, d_dy, d_x, d_dw, d_workspace, workspace_bytes, &p);
+    if (!why.empty()) return fail(ctx, SRF_ERR_ARG, why);
+    DeviceGuard guard(ctx->device);
+    if (workspace_bytes < grouped_weight_grad_workspace(p, sm_count()))
+        return fail(ctx, SRF_ERR_CAPACITY, "d_workspace is smaller than srf_grouped_weight_grad_workspace says");
+    return launched(ctx, launch_grouped_weight_grad(p, d_offsets, d_dy, d_x, d_dw, d_workspace, &ctx->d_counters->error_flags, (cudaStream_t)stream));
+}
+
+srf_status srf_grouped_matmul_fp8(srf_ctx* ctx, const srf_grouped_t* in, const uint64_t* d_offsets, const void* d_x, const float* d_x_scales,
+                                  const void* d_w, const float* d_w_scales, void* d_y, void* stream) {
+    if (!ctx) return SRF_ERR_ARG;
+    srf_grouped_t p;
+    const std::string why = refuse_matmul_fp8(in, d_offsets, d_x, d_x_scales, d_w, d_w_scales, d_y, &p);
+    if (!why.empty()) return fail(ctx, SRF_ERR_ARG, why);
+    DeviceGuard guard(ctx->device);
+    return launched(ctx, launch_grouped_matmul_fp8(p, d_offsets, d_x, d_x_scales, d_w, d_w_scales, d_y, &ctx->d_counters->error_flags, (cudaStream_t)stream));
+}
+
+srf_status srf_quantize_rows(srf_ctx* ctx, int type, uint64_t n_rows, const uint64_t* d_n_rows_used, uint32_t n_cols, const void* d_in,
+                             uint64_t ld_in, void* d_out, uint64_t ld_out, float* d_scales, void* stream) {
+    if (!ctx) return SRF_ERR_ARG;
+    const std::string why = refuse_quantize_rows(type, n_rows, d_n_rows_used, n_cols, d_in, &ld_in, d_out, &ld_out, d_scales);
+    if (!why.empty()) return fail(ctx, SRF_ERR_ARG, why);
+    DeviceGuard guard(ctx->device);
+    launch_quantize_rows(type, n_rows, d_n_rows_used, n_cols, d_in, ld_in, d_out, ld_out, d_scales, (cudaStream_t)stream);
+    return launched(ctx, nullptr);
+}
+
+srf_status srf_quantize_weights(srf_ctx* ctx, int type, uint32_t n_matrices, uint32_t n_rows, uint32_t n_cols, const void* d_in,
+                                uint64_t ld_in, void* d_out, uint64_t ld_out, float* d_scales, void* stream) {
+    if (!ctx) return SRF_ERR_ARG;
+    const std::string why = refuse_quantize_weights(type, n_matrices, n_rows, n_cols, d_in, &ld_in, d_out, &ld_out, d_scales);
+    if (!why.empty()) return fail(ctx, SRF_ERR_ARG, why);
+    DeviceGuard guard(ctx->device);
+    launch_quantize_weights(type, n_matrices, n_rows, n_cols, d_in, ld_in, n_rows * ld_in, d_out, ld_out, n_rows * ld_out, d_scales, (cudaStream_t)stream);
+    return launched(ctx, nullptr);
 }
 
 srf_status srf_volume_rendering(srf_ctx* ctx, const srf_view_t* view, const uint64_t* d_offsets, uint64_t n_rays,

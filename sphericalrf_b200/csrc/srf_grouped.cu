@@ -1,0 +1,542 @@
+// srf_grouped.cu -- matrix products grouped by ragged sample lists, 16-bit values, on tcgen05 / TMEM.
+//
+// The samples of a frame or batch are sorted by region; group g owns samples offsets[g] .. offsets[g+1] and a matrix
+// W[g] (n_out x n_in, row-major like the network's own layers).  Three products, all D = A B^T summed over k:
+//
+//   layer        y[r][n]  = act(sum_k x[r][k]  W[g][n][k])    A = samples, k = inputs    B = W[g]
+//   input grad   dx[r][k] = sum_n dy[r][n] W[g][n][k]         A = samples, k = outputs   B = W[g], read down its columns
+//   weight grad  dW[g][n][k] = sum_r dy[r][n] x[r][k]         A, B = both sample arrays, read down their columns
+//
+// One persistent CTA per SM: a TMA warp fills a ring of 64-deep operand stages, one thread issues tcgen05.mma
+// (M = 128, N = BN, fp32 accumulator in TMEM, two accumulators), four warps take a finished accumulator to memory while
+// the next one fills.  Operands that are read down their columns stay as they lie in memory: the tensor core takes them
+// MN-major.  Tiles are dealt round-robin; every warp finds its tiles itself from the offsets (GroupWalk), so no launch,
+// workspace or host read prepares them.
+//
+// A tile's rows behind its group's end hold the next group's samples: harmless in the first two products (an output row
+// depends on its own sample alone and those rows are not stored).  In the weight gradient they would be summed, so the
+// rows of the last stage of a group are zeroed in shared memory, in both operands (a NaN of the next group must not
+// meet a zero).
+#include <cstdio>
+#include <cstring>
+#include "srf_layers.cuh"
+#include "srf_tile.cuh"
+
+namespace srf {
+
+using namespace tile;
+
+namespace {
+
+enum Mode { kLayer = 0, kInputGrad = 1, kWeightGrad = 2 };
+
+constexpr int kThreads = 256;                 // TMA, MMA, TMEM owner, spare, 4 epilogue warps
+constexpr int kBM = 128, kBK = 64;
+constexpr uint32_t kTmemCols = 512;
+constexpr int kABytes = kBM * kBK * 2;
+constexpr int kStoreBytes = 4 * 4096;         // staging of the four epilogue warps
+constexpr int kSmemMin = 120 * 1024;          // a second CTA that allocates TMEM must never share the SM
+
+struct GroupedArgs {
+    const uint64_t* offsets;
+    unsigned char* out;
+    const unsigned char* gate;
+    float* partial;               // weight gradient: two tiles of partial sums per CTA
+    uint64_t n_rows;
+    uint64_t out_row_bytes, out_group_bytes, gate_row_bytes;
+    uint32_t n_groups;
+    uint32_t out_rows;            // weight gradient: n_out
+    uint32_t out_cols;            // n_out, n_in, n_in
+    uint32_t depth;               // summed length of the first two products
+    int bf16, f32, relu;
+    unsigned int* error_flags;
+};
+
+template <int BN>
+__host__ __device__ constexpr int n_stages() { return BN == 256 ? 4 : BN == 128 ? 6 : 8; }
+template <int BN>
+__host__ __device__ constexpr int smem_bytes() {
+    const int b = 1024 + n_stages<BN>() * (kABytes + BN * kBK * 2) + kStoreBytes + 512;
+    return b < kSmemMin ? kSmemMin : b;
+}
+
+// Units of work of a group: whole output tiles for the first two products; 64-sample stages of output tiles for the
+// weight gradient, whose work is cut evenly across the CTAs (see below).
+template <int MODE>
+__device__ __forceinline__ uint64_t group_units(const Span& s, uint32_t tiles_across) {
+    const uint64_t rows = s.end - s.begin;
+    return (MODE == kWeightGrad ? (rows + kBK - 1) / kBK : (rows + kBM - 1) / kBM) * tiles_across;
+}
+
+// One stretch of summed stages of one output tile.
+struct Piece {
+    uint32_t group;
+    Span span;
+    uint64_t m;            // first output row: sample (first two products) or row of W (weight gradient)
+    uint32_t n;            // output column tile
+    uint64_t k0;           // first stage
+    uint64_t k_stages;     // stages
+    bool whole;            // the piece is the tile's whole sum
+    bool first;            // the piece holds the tile's first stage
+};
+
+// The pieces of this CTA, one after the other; every warp walks them for itself.
+//
+// Weight gradient: the stages of all tiles are one line of `units` which the CTAs share out evenly, so ragged groups
+// balance by themselves and a narrow layer (one tile per group) still fills every SM.  A tile that a boundary cuts
+// is summed from the CTAs' partial sums, in the CTAs' order, by a second kernel: the same result on every run.
+template <int MODE>
+struct Pieces {
+    GroupWalk walk;
+    uint64_t at, stop;
+    __device__ __forceinline__ void init(uint64_t units) {
+        if (MODE == kWeightGrad) {
+            const uint64_t q = units / gridDim.x, r = units % gridDim.x;
+            at = blockIdx.x * q + (blockIdx.x < r ? blockIdx.x : r);
+            stop = at + q + (blockIdx.x < r ? 1 : 0);
+        } else {
+            at = blockIdx.x;
+            stop = ~0ull;
+        }
+    }
+    __device__ __forceinline__ bool next(const GroupedArgs& p, uint32_t tiles_m, uint32_t tiles_n, Piece* o, bool* bad) {
+        if (at >= stop) return false;
+        const uint32_t across = MODE == kWeightGrad ? tiles_m * tiles_n : tiles_n;
+        uint64_t local;
+        if (!walk.find(at, p.offsets, p.n_groups, p.n_rows, [&](const Span& s) { return group_units<MODE>(s, across); },
+                       &o->group, &o->span, &local, bad))
+            return false;
+        const uint64_t rows = o->span.end - o->span.begin;
+        if (MODE == kWeightGrad) {
+            const uint64_t deep = (rows + kBK - 1) / kBK;
+            const uint64_t t = local / deep;
+            uint64_t m;
+            tile_place(t, tiles_m, tiles_n, &m, &o->n);
+            o->m = m * kBM;
+            o->k0 = local - t * deep;
+            o->k_stages = deep - o->k0 < stop - at ? deep - o->k0 : stop - at;
+            o->first = o->k0 == 0;
+            o->whole = o->k_stages == deep;
+            at += o->k_stages;
+        } else {
+            uint64_t m;
+            tile_place(local, (rows + kBM - 1) / kBM, tiles_n, &m, &o->n);
+            o->m = o->span.begin + m * kBM;
+            o->k0 = 0;
+            o->k_stages = (p.depth + kBK - 1) / kBK;
+            o->first = o->whole = true;
+            at += gridDim.x;
+        }
+        return true;
+    }
+};
+
+// Units of all groups (warp-collective).
+template <int MODE>
+__device__ __forceinline__ uint64_t all_units(const GroupedArgs& p, uint32_t across, bool* bad) {
+    uint64_t sum = 0;
+    for (uint32_t g = threadIdx.x & 31; g < p.n_groups; g += 32) sum += group_units<MODE>(group_span(p.offsets, g, p.n_rows, bad), across);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    return sum;
+}
+
+template <int MODE, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GroupedArgs p) {
+    constexpr int kStages = n_stages<BN>();
+    constexpr int kBBytes = BN * kBK * 2;
+    constexpr bool kAColumns = MODE == kWeightGrad, kBColumns = MODE != kLayer;     // read down the columns: MN-major
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    unsigned char* sm_a = smem;
+    unsigned char* sm_b = smem + kStages * kABytes;
+    unsigned char* sm_store = sm_b + kStages * kBBytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm_store + kStoreBytes);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
+    volatile uint32_t* failed = tmem_slot + 1;
+    const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kStages;
+    const uint32_t bar_acc_full = bar_empty + 8 * kStages, bar_acc_empty = bar_acc_full + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t tiles_n = (p.out_cols + BN - 1) / BN;
+    const uint32_t tiles_m = MODE == kWeightGrad ? (p.out_rows + kBM - 1) / kBM : 0;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(bar_acc_full + 8 * i, 1); mbar_init(bar_acc_empty + 8 * i, 4); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        *failed = 0;
+        tma_prefetch_map(&map_a);
+        tma_prefetch_map(&map_b);
+    }
+    if (warp == 2) tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    bool bad = false, ok = true;
+    Pieces<MODE> pieces;
+    pieces.init(MODE == kWeightGrad ? all_units<MODE>(p, tiles_m * tiles_n, &bad) : 0);
+    Piece t;
+
+    if (warp == 0) {
+        // ---- operand loads ----
+        uint32_t s = 0, round = 0;                     // ring position
+        uint32_t in_flight = 0;
+        while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
+            for (uint64_t k = 0; k < t.k_stages; ++k) {
+                if (round > 0 && !mbar_wait(bar_empty + 8 * s, (round - 1) & 1, failed)) { ok = false; break; }
+                if (elect_one()) {
+                    const uint32_t bar = bar_full + 8 * s, a = smem_u32(sm_a) + s * kABytes, b = smem_u32(sm_b) + s * kBBytes;
+                    mbar_expect(bar, kABytes + kBBytes);
+                    const int kk = (int)((t.k0 + k) * kBK);
+                    if (kAColumns) {
+#pragma unroll
+                        for (int i = 0; i < kBM / 64; ++i) tma_2d(a + i * 8192, &map_a, bar, (int)t.m + 64 * i, (int)t.span.begin + kk);
+                    } else {
+                        tma_2d(a, &map_a, bar, kk, (int)t.m);
+                    }
+                    if (MODE == kLayer) {
+                        tma_3d(b, &map_b, bar, kk, (int)(t.n * BN), (int)t.group);
+                    } else if (MODE == kInputGrad) {
+#pragma unroll
+                        for (int i = 0; i < BN / 64; ++i) tma_3d(b + i * 8192, &map_b, bar, (int)(t.n * BN) + 64 * i, kk, (int)t.group);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < BN / 64; ++i) tma_2d(b + i * 8192, &map_b, bar, (int)(t.n * BN) + 64 * i, (int)t.span.begin + kk);
+                    }
+                }
+                __syncwarp();
+                if (++s == kStages) { s = 0; ++round; }
+                in_flight = in_flight < kStages ? in_flight + 1 : in_flight;
+            }
+        }
+        // Copies may still be on their way when another warp gave up: they must land before the CTA leaves.
+        if (!ok || *failed) {
+            for (uint32_t i = 0; i < in_flight; ++i) {
+                const uint32_t q = s >= i + 1 ? s - i - 1 : s + kStages - i - 1;
+                const uint32_t r = s >= i + 1 ? round : round - 1;
+                uint32_t none = 0;
+                mbar_wait(bar_full + 8 * q, r & 1, &none);
+            }
+        }
+    } else if (warp == 1) {
+        // ---- matrix instructions ----
+        const uint32_t idesc = idesc_shape(BN) | (p.bf16 ? (1u << 7) | (1u << 10) : 0u) | (kAColumns ? 1u << 15 : 0u) | (kBColumns ? 1u << 16 : 0u);
+        uint32_t s = 0, round = 0, acc = 0, acc_round = 0;
+        while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
+            if (acc_round > 0 && !mbar_wait(bar_acc_empty + 8 * acc, (acc_round - 1) & 1, failed)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t d = tmem + acc * 256;
+            for (uint64_t k = 0; k < t.k_stages; ++k) {
+                if (!mbar_wait(bar_full + 8 * s, round & 1, failed)) { ok = false; break; }
+                tc_fence_after();
+                int k_steps = kBK / 16;
+                if (MODE == kWeightGrad) {
+                    const uint64_t left = t.span.end - t.span.begin - (t.k0 + k) * kBK;     // samples of this stage
+                    if (left < (uint64_t)kBK) {
+                        // the group's last stage: instructions cover whole 16s, so zero up to the next 16
+                        const int r0 = (int)left, r1 = (r0 + 15) & ~15;
+                        k_steps = r1 / 16;
+                        const int units = (r1 - r0) * 8;
+                        for (int i = lane; i < units * (kBM / 64 + BN / 64); i += 32) {
+                            const int blk = i / units, u = i - blk * units;
+                            unsigned char* base = blk < kBM / 64 ? sm_a + s * kABytes + blk * 8192 : sm_b + s * kBBytes + (blk - kBM / 64) * 8192;
+                            *reinterpret_cast<uint4*>(base + r0 * 128 + u * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        fence_async_smem();
+                        __syncwarp();
+                    }
+                }
+                if (elect_one()) {
+                    const uint32_t a = smem_u32(sm_a) + s * kABytes, b = smem_u32(sm_b) + s * kBBytes;
+                    for (int q = 0; q < k_steps; ++q) {
+                        const uint64_t da = kAColumns ? operand_desc(a + q * 2048, 8192, 1024) : operand_desc(a + q * 32, 16, 1024);
+                        const uint64_t db = kBColumns ? operand_desc(b + q * 2048, 8192, 1024) : operand_desc(b + q * 32, 16, 1024);
+                        mma_f16(d, da, db, idesc, (k | (uint64_t)q) != 0);
+                    }
+                    mma_commit(bar_empty + 8 * s);
+                    if (k + 1 == t.k_stages) mma_commit(bar_acc_full + 8 * acc);
+                }
+                __syncwarp();
+                if (++s == kStages) { s = 0; ++round; }
+            }
+            if (!ok) break;
+            if (++acc == 2) { acc = 0; ++acc_round; }
+        }
+    } else if (warp >= 4) {
+        // ---- finished accumulators to memory ----
+        const int quarter = warp & 3;
+        unsigned char* stage = sm_store + quarter * 4096;
+        uint32_t acc = 0, acc_round = 0;
+        while (pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
+            if (!mbar_wait(bar_acc_full + 8 * acc, acc_round & 1, failed)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t d = tmem + acc * 256 + ((uint32_t)(quarter * 32) << 16);
+            RowStore rs;
+            rs.bf16 = p.bf16 != 0;
+            rs.gate = nullptr;
+            rs.gate_row_bytes = p.gate_row_bytes;
+            const bool partial = MODE == kWeightGrad && !t.whole;
+            rs.f32 = partial || p.f32;
+            const uint64_t row0 = t.m + (uint64_t)quarter * 32;
+            const uint64_t end = MODE == kWeightGrad ? (uint64_t)p.out_rows : t.span.end;
+            rs.rows = row0 >= end ? 0u : end - row0 < 32 ? (uint32_t)(end - row0) : 32u;
+            const uint32_t col0 = t.n * BN;
+            const uint32_t cols = p.out_cols - col0 < (uint32_t)BN ? p.out_cols - col0 : (uint32_t)BN;
+            unsigned char* out;
+            if (partial) {
+                // slot 0: the tile began in an earlier CTA; slot 1: it goes on in the next one
+                out = reinterpret_cast<unsigned char*>(p.partial + ((size_t)blockIdx.x * 2 + (t.first ? 1 : 0)) * kBM * BN) + (size_t)quarter * 32 * BN * 4;
+                rs.row_bytes = BN * 4;
+            } else {
+                out = p.out + (MODE == kWeightGrad ? t.group * p.out_group_bytes : 0ull) + row0 * p.out_row_bytes;
+                rs.row_bytes = p.out_row_bytes;
+            }
+            const uint32_t per = rs.f32 ? 32u : 64u;
+            for (uint32_t c = 0; c < cols; c += per) {
+                uint32_t r[32];
+                if (rs.f32) {
+                    tmem_ld32(d + c, r);
+                    tmem_ld_wait();
+                    if (p.relu)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(relu(__uint_as_float(r[i])));
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) stage_unit(stage, lane, u, make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]));
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (c + 32u * h < cols) {
+                            tmem_ld32(d + c + 32 * h, r);
+                            tmem_ld_wait();
+                            if (p.relu)
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(relu(__uint_as_float(r[i])));
+                            uint32_t o[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = pack16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), rs.bf16);
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) stage_unit(stage, lane, 4 * h + u, make_uint4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]));
+                        }
+                    }
+                }
+                if (c + per >= cols) {             // the accumulator is read: the next tile may have it
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_acc_empty + 8 * acc);
+                }
+                const uint32_t size = rs.f32 ? 4u : 2u;
+                rs.bytes = (cols - c < per ? cols - c : per) * size;
+                rs.out = out + (size_t)(partial ? c : col0 + c) * size;
+                if (MODE == kInputGrad && p.gate) rs.gate = p.gate + row0 * p.gate_row_bytes + (size_t)(col0 + c) * 2;
+                store_rows(rs, stage);
+            }
+            if (++acc == 2) { acc = 0; ++acc_round; }
+        }
+    }
+    if ((bad || (!ok && lane == 0)) && p.error_flags) atomicOr(p.error_flags, (ok ? 0u : 2u) | (bad ? 16u : 0u));
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) tmem_free(tmem, kTmemCols);
+}
+
+// Second kernel of the weight gradient.  Block (tile, group, slice of 16 rows): sums the partial tiles of an output
+// tile that more than one CTA worked on, in the CTAs' order, or writes the zeros of a group without samples.
+template <int BN>
+__global__ void __launch_bounds__(256) k_weight_grad_join(const GroupedArgs p, uint32_t n_ctas) {
+    const uint32_t tiles_n = (p.out_cols + BN - 1) / BN, tiles_m = (p.out_rows + kBM - 1) / kBM;
+    const uint32_t across = tiles_m * tiles_n;
+    const uint32_t g = blockIdx.y, tile_id = blockIdx.x / (kBM / 16), slice = blockIdx.x % (kBM / 16);
+    __shared__ uint64_t sh_units[2];
+    bool bad = false;
+    if (threadIdx.x < 32) {
+        uint64_t all = 0, before = 0;
+        for (uint32_t q = threadIdx.x; q < p.n_groups; q += 32) {
+            const uint64_t u = group_units<kWeightGrad>(group_span(p.offsets, q, p.n_rows, &bad), across);
+            all += u;
+            if (q < g) before += u;
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            all += __shfl_xor_sync(0xffffffffu, all, d);
+            before += __shfl_xor_sync(0xffffffffu, before, d);
+        }
+        if (threadIdx.x == 0) { sh_units[0] = all; sh_units[1] = before; }
+    }
+    __syncthreads();
+    const Span s = group_span(p.offsets, g, p.n_rows, &bad);
+    const uint64_t deep = (s.end - s.begin + kBK - 1) / kBK;
+    uint32_t c0 = 0, c1 = 0;
+    if (deep) {
+        // CTA c works on units [c q + min(c, r), ...): the owners of the tile's first and last unit
+        const uint64_t q = sh_units[0] / n_ctas, r = sh_units[0] % n_ctas;
+        const uint64_t u0 = sh_units[1] + tile_id * deep, u1 = u0 + deep - 1;
+        auto owner = [&](uint64_t u) { return (uint32_t)(u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q); };
+        c0 = owner(u0);
+        c1 = owner(u1);
+        if (c0 == c1) return;
+    }
+    uint64_t m;
+    uint32_t n;
+    tile_place(tile_id, tiles_m, tiles_n, &m, &n);
+    for (uint32_t i = threadIdx.x; i < 16 * BN; i += blockDim.x) {
+        const uint32_t row = slice * 16 + i / BN, col = i % BN;
+        const uint64_t orow = m * kBM + row;
+        const uint32_t ocol = n * BN + col;
+        if (orow >= p.out_rows || ocol >= p.out_cols) continue;
+        float sum = 0.f;
+        if (deep) {
+            sum = p.partial[((size_t)c0 * 2 + 1) * kBM * BN + (size_t)row * BN + col];
+            for (uint32_t c = c0 + 1; c <= c1; ++c) sum += p.partial[(size_t)c * 2 * kBM * BN + (size_t)row * BN + col];
+        }
+        unsigned char* o = p.out + g * p.out_group_bytes + orow * p.out_row_bytes;
+        if (p.f32) reinterpret_cast<float*>(o)[ocol] = sum;
+        else reinterpret_cast<uint16_t*>(o)[ocol] = (uint16_t)pack16(sum, 0.f, p.bf16 != 0);
+    }
+}
+
+// Width of the output tile: the widest that leaves every SM a few tiles (a wide tile reads its operands from L2 less
+// often, a narrow one spreads few tiles over more SMs).
+int pick_bn(uint64_t row_tiles, uint32_t cols, int sms, int smallest) {
+    int bn = 256;
+    while (bn > smallest && (((uint64_t)(bn / 2) >= cols) || row_tiles * ((cols + bn - 1) / bn) < 2ull * sms)) bn /= 2;
+    return bn;
+}
+
+template <int MODE, int BN>
+const char* launch(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& args, uint64_t max_units, cudaStream_t stream) {
+    static_assert(smem_bytes<BN>() <= 227 * 1024, "shared memory of one SM");
+    const int sms = sm_count();
+    if (cudaFuncSetAttribute((const void*)k_grouped<MODE, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<BN>()) != cudaSuccess)
+        return "cudaFuncSetAttribute failed";
+    const int grid = (int)(max_units < (uint64_t)sms ? max_units : (uint64_t)sms);
+    k_grouped<MODE, BN><<<grid, kThreads, smem_bytes<BN>(), stream>>>(a, b, args);
+    return nullptr;
+}
+
+// Row tiles that n_rows samples in n_groups groups can have at most.
+uint64_t max_row_tiles(const srf_grouped_t& p) {
+    const uint64_t busy = p.n_groups < p.n_rows ? p.n_groups : p.n_rows;
+    return p.n_rows / kBM + busy;
+}
+
+int weight_grad_bn(const srf_grouped_t& p) { return p.n_in <= 64 ? 64 : p.n_in <= 128 ? 128 : 256; }
+
+}  // namespace
+
+int sm_count() {
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return sms;
+}
+
+bool make_operand_map(void* map, const void* base, int type, uint64_t cols, uint64_t rows, uint64_t ld, uint64_t n_matrices,
+                      uint64_t matrix_stride, uint32_t box_rows) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<Encode>(f);
+    }();
+    if (!encode) return false;
+    const uint64_t size = type == SRF_TYPE_E4M3 ? 1 : 2;
+    const cuuint32_t rank = n_matrices ? 3 : 2;
+    const cuuint64_t dims[3] = {cols, rows, n_matrices};
+    const cuuint64_t strides[2] = {ld * size, matrix_stride * size};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / size), box_rows, 1};
+    const cuuint32_t step[3] = {1, 1, 1};
+    const CUtensorMapDataType dt = type == SRF_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : type == SRF_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    return encode(reinterpret_cast<CUtensorMap*>(map), dt, rank, const_cast<void*>(base), dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+const char* launch_grouped_matmul(const srf_grouped_t& p, const uint64_t* offsets, const void* x, const void* w, void* y,
+                                  unsigned int* error_flags, cudaStream_t stream) {
+    const uint64_t row_tiles = max_row_tiles(p);
+    if (!row_tiles) return nullptr;
+    const int bn = pick_bn(row_tiles, p.n_out, sm_count(), 32);
+    CUtensorMap a, b;
+    if (!make_operand_map(&a, x, p.type, p.n_in, p.n_rows, p.ld_x, 0, 0, kBM) ||
+        !make_operand_map(&b, w, p.type, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, bn))
+        return "the driver refused an operand's tensor map";
+    GroupedArgs k;
+    memset(&k, 0, sizeof(k));
+    k.offsets = offsets; k.out = (unsigned char*)y; k.n_rows = p.n_rows; k.n_groups = p.n_groups;
+    k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16; k.relu = p.activation == SRF_ACT_RELU;
+    k.out_row_bytes = p.ld_y * (k.f32 ? 4 : 2); k.out_cols = p.n_out; k.depth = p.n_in; k.error_flags = error_flags;
+    const uint64_t units = row_tiles * ((p.n_out + bn - 1) / bn);
+    switch (bn) {
+    case 256: return launch<kLayer, 256>(a, b, k, units, stream);
+    case 128: return launch<kLayer, 128>(a, b, k, units, stream);
+    case 64: return launch<kLayer, 64>(a, b, k, units, stream);
+    default: return launch<kLayer, 32>(a, b, k, units, stream);
+    }
+}
+
+const char* launch_grouped_input_grad(const srf_grouped_t& p, const uint64_t* offsets, const void* dy, const void* w,
+                                      const void* gate, void* dx, unsigned int* error_flags, cudaStream_t stream) {
+    const uint64_t row_tiles = max_row_tiles(p);
+    if (!row_tiles) return nullptr;
+    const int bn = pick_bn(row_tiles, p.n_in, sm_count(), 64);
+    CUtensorMap a, b;
+    if (!make_operand_map(&a, dy, p.type, p.n_out, p.n_rows, p.ld_y, 0, 0, kBM) ||
+        !make_operand_map(&b, w, p.type, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, kBK))
+        return "the driver refused an operand's tensor map";
+    GroupedArgs k;
+    memset(&k, 0, sizeof(k));
+    k.offsets = offsets; k.out = (unsigned char*)dx; k.gate = (const unsigned char*)gate; k.n_rows = p.n_rows; k.n_groups = p.n_groups;
+    k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16;
+    k.out_row_bytes = p.ld_x * (k.f32 ? 4 : 2); k.gate_row_bytes = p.ld_x * 2; k.out_cols = p.n_in; k.depth = p.n_out;
+    k.error_flags = error_flags;
+    const uint64_t units = row_tiles * ((p.n_in + bn - 1) / bn);
+    switch (bn) {
+    case 256: return launch<kInputGrad, 256>(a, b, k, units, stream);
+    case 128: return launch<kInputGrad, 128>(a, b, k, units, stream);
+    default: return launch<kInputGrad, 64>(a, b, k, units, stream);
+    }
+}
+
+size_t grouped_weight_grad_workspace(const srf_grouped_t& p, int n_sms) {
+    return (size_t)n_sms * 2 * kBM * weight_grad_bn(p) * sizeof(float);
+}
+
+const char* launch_grouped_weight_grad(const srf_grouped_t& p, const uint64_t* offsets, const void* dy, const void* x, void* dw,
+                                       void* workspace, unsigned int* error_flags, cudaStream_t stream) {
+    const int bn = weight_grad_bn(p);
+    GroupedArgs k;
+    memset(&k, 0, sizeof(k));
+    k.offsets = offsets; k.out = (unsigned char*)dw; k.partial = (float*)workspace; k.n_rows = p.n_rows; k.n_groups = p.n_groups;
+    k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16;
+    k.out_row_bytes = p.ld_w * (k.f32 ? 4 : 2); k.out_group_bytes = p.group_stride * (k.f32 ? 4 : 2);
+    k.out_rows = p.n_out; k.out_cols = p.n_in; k.error_flags = error_flags;
+    const uint64_t across = (uint64_t)((p.n_out + kBM - 1) / kBM) * ((p.n_in + bn - 1) / bn);
+    const uint64_t busy = p.n_groups < p.n_rows ? p.n_groups : p.n_rows;
+    const uint64_t units = (p.n_rows / kBK + busy) * across;
+    const int sms = sm_count();
+    const uint32_t grid = (uint32_t)(units < (uint64_t)sms ? units : (uint64_t)sms);
+    if (units) {
+        CUtensorMap a, b;
+        if (!make_operand_map(&a, dy, p.type, p.n_out, p.n_rows, p.ld_y, 0, 0, kBK) ||
+            !make_operand_map(&b, x, p.type, p.n_in, p.n_rows, p.ld_x, 0, 0, kBK))
+            return "the driver refused an operand's tensor map";
+        const char* why = bn == 256 ? launch<kWeightGrad, 256>(a, b, k, units, stream)
+                        : bn == 128 ? launch<kWeightGrad, 128>(a, b, k, units, stream)
+                                    : launch<kWeightGrad, 64>(a, b, k, units, stream);
+        if (why) return why;
+    }
+    const dim3 join_grid((uint32_t)(across * (kBM / 16)), p.n_groups);
+    const uint32_t n_ctas = grid ? grid : 1;
+    if (bn == 256) k_weight_grad_join<256><<<join_grid, 256, 0, stream>>>(k, n_ctas);
+    else if (bn == 128) k_weight_grad_join<128><<<join_grid, 256, 0, stream>>>(k, n_ctas);
+    else k_weight_grad_join<64><<<join_grid, 256, 0, stream>>>(k, n_ctas);
+    return nullptr;
+}
+
+}  // namespace srf

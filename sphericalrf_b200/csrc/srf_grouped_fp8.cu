@@ -1,0 +1,268 @@
+// srf_grouped_fp8.cu -- the grouped layer on 8-bit (e4m3) samples and weights, on tcgen05 / TMEM.
+//
+//   y[r][n] = act( sum_b sx[b][r] sw[g][n/128][b] * sum_{k in block b} x[r][k] W[g][n][k] ),   blocks of 128 inputs
+//
+// Inside a block the tensor core sums products of 8-bit values in fp32 (TMEM); the scales differ from block to block, so
+// every block's sum is taken out of TMEM, scaled and added in fp32 registers.  A stage of the operand ring is one block
+// (128 bytes of every row), its four instructions start a new accumulator, and two warpgroups -- each half of the tile's
+// columns -- follow one block behind.  The rest is as in srf_grouped.cu.
+#include <cstring>
+#include "srf_layers.cuh"
+#include "srf_tile.cuh"
+
+namespace srf {
+
+using namespace tile;
+
+namespace {
+
+constexpr int kThreads = 384;                 // TMA, MMA, TMEM owner, spare, 8 scaling warps
+constexpr int kBM = 128, kBK = 128;
+constexpr uint32_t kTmemCols = 512;
+constexpr int kABytes = kBM * kBK;
+constexpr int kStoreBytes = 8 * 4096;
+constexpr int kSmemMin = 120 * 1024;          // a second CTA that allocates TMEM must never share the SM
+
+struct Fp8Args {
+    const uint64_t* offsets;
+    unsigned char* out;
+    const float* x_scales;        // [blocks of n_in][n_rows]
+    const float* w_scales;        // [group][blocks of n_out][blocks of n_in]
+    uint64_t n_rows, out_row_bytes;
+    uint32_t n_groups, n_in, n_out;
+    int bf16, f32, relu;
+    unsigned int* error_flags;
+};
+
+template <int BN> __host__ __device__ constexpr int n_stages() { return BN == 256 ? 3 : BN == 128 ? 5 : 6; }
+template <int BN> __host__ __device__ constexpr int n_accs() { return BN == 256 ? 2 : 4; }
+template <int BN>
+__host__ __device__ constexpr int smem_bytes() {
+    const int b = 1024 + n_stages<BN>() * (kABytes + BN * kBK) + kStoreBytes + 512;
+    return b < kSmemMin ? kSmemMin : b;
+}
+
+template <int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Fp8Args p) {
+    constexpr int kStages = n_stages<BN>(), kAccs = n_accs<BN>();
+    constexpr int kBBytes = BN * kBK;
+    constexpr int kCols = BN / 2;                 // columns of one warpgroup
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    unsigned char* sm_a = smem;
+    unsigned char* sm_b = smem + kStages * kABytes;
+    unsigned char* sm_store = sm_b + kStages * kBBytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm_store + kStoreBytes);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2 * kAccs);
+    volatile uint32_t* failed = tmem_slot + 1;
+    const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kStages;
+    const uint32_t bar_acc_full = bar_empty + 8 * kStages, bar_acc_empty = bar_acc_full + 8 * kAccs;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t tiles_n = (p.n_out + BN - 1) / BN;
+    const uint32_t blocks_k = (p.n_in + kBK - 1) / kBK, blocks_n = (p.n_out + 127) / 128;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
+        for (int i = 0; i < kAccs; ++i) { mbar_init(bar_acc_full + 8 * i, 1); mbar_init(bar_acc_empty + 8 * i, 8); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        *failed = 0;
+        tma_prefetch_map(&map_a);
+        tma_prefetch_map(&map_b);
+    }
+    if (warp == 2) tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    bool bad = false, ok = true;
+    GroupWalk walk;
+    uint64_t at = blockIdx.x;
+    uint32_t group = 0, tn = 0;
+    uint64_t m = 0;
+    Span span = {0, 0};
+    auto next_tile = [&]() -> bool {
+        uint64_t local;
+        if (!walk.find(at, p.offsets, p.n_groups, p.n_rows,
+                       [&](const Span& s) { return (s.end - s.begin + kBM - 1) / kBM * tiles_n; }, &group, &span, &local, &bad))
+            return false;
+        tile_place(local, (span.end - span.begin + kBM - 1) / kBM, tiles_n, &m, &tn);
+        m = span.begin + m * kBM;
+        at += gridDim.x;
+        return true;
+    };
+
+    if (warp == 0) {
+        // ---- operand loads ----
+        uint32_t s = 0, round = 0, in_flight = 0;
+        while (ok && next_tile()) {
+            for (uint32_t k = 0; k < blocks_k; ++k) {
+                if (round > 0 && !mbar_wait(bar_empty + 8 * s, (round - 1) & 1, failed)) { ok = false; break; }
+                if (elect_one()) {
+                    const uint32_t bar = bar_full + 8 * s;
+                    mbar_expect(bar, kABytes + kBBytes);
+                    tma_2d(smem_u32(sm_a) + s * kABytes, &map_a, bar, (int)(k * kBK), (int)m);
+                    tma_3d(smem_u32(sm_b) + s * kBBytes, &map_b, bar, (int)(k * kBK), (int)(tn * BN), (int)group);
+                }
+                __syncwarp();
+                if (++s == kStages) { s = 0; ++round; }
+                in_flight = in_flight < kStages ? in_flight + 1 : in_flight;
+            }
+        }
+        // Copies may still be on their way when another warp gave up: they must land before the CTA leaves.
+        if (!ok || *failed) {
+            for (uint32_t i = 0; i < in_flight; ++i) {
+                const uint32_t q = s >= i + 1 ? s - i - 1 : s + kStages - i - 1;
+                const uint32_t r = s >= i + 1 ? round : round - 1;
+                uint32_t none = 0;
+                mbar_wait(bar_full + 8 * q, r & 1, &none);
+            }
+        }
+    } else if (warp == 1) {
+        // ---- matrix instructions: four to a block, each block its own accumulator ----
+        constexpr uint32_t idesc = idesc_shape(BN);      // e4m3 is format 0
+        uint32_t s = 0, round = 0, acc = 0, acc_round = 0;
+        while (ok && next_tile()) {
+            for (uint32_t k = 0; k < blocks_k; ++k) {
+                if (acc_round > 0 && !mbar_wait(bar_acc_empty + 8 * acc, (acc_round - 1) & 1, failed)) { ok = false; break; }
+                if (!mbar_wait(bar_full + 8 * s, round & 1, failed)) { ok = false; break; }
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t a = smem_u32(sm_a) + s * kABytes, b = smem_u32(sm_b) + s * kBBytes;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        mma_f8(tmem + acc * BN, operand_desc(a + q * 32, 16, 1024), operand_desc(b + q * 32, 16, 1024), idesc, q != 0);
+                    mma_commit(bar_empty + 8 * s);
+                    mma_commit(bar_acc_full + 8 * acc);
+                }
+                __syncwarp();
+                if (++s == kStages) { s = 0; ++round; }
+                if (++acc == kAccs) { acc = 0; ++acc_round; }
+            }
+        }
+    } else if (warp >= 4) {
+        // ---- scale, sum, store ----
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        unsigned char* stage = sm_store + (warp - 4) * 4096;
+        uint32_t acc = 0, acc_round = 0;
+        while (ok && next_tile()) {
+            const uint64_t row0 = m + (uint64_t)quarter * 32;
+            const uint64_t row = row0 + lane < p.n_rows ? row0 + lane : p.n_rows - 1;
+            const uint32_t col0 = tn * BN + half * kCols;
+            const uint32_t wb = col0 / 128 < blocks_n ? col0 / 128 : blocks_n - 1;
+            const float* sx = p.x_scales + row;
+            const float* sw = p.w_scales + ((size_t)group * blocks_n + wb) * blocks_k;
+            float sum[kCols];
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) sum[i] = 0.f;
+            float scale = __ldg(sx) * __ldg(sw);
+            for (uint32_t k = 0; k < blocks_k; ++k) {
+                float ahead = 0.f;
+                if (k + 1 < blocks_k) ahead = __ldg(sx + (size_t)(k + 1) * p.n_rows) * __ldg(sw + k + 1);
+                if (!mbar_wait(bar_acc_full + 8 * acc, acc_round & 1, failed)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t d = tmem + acc * BN + half * kCols + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll
+                for (int c = 0; c < kCols; c += 32) {
+                    uint32_t r[32];
+                    tmem_ld32(d + c, r);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[c + i] = fmaf(__uint_as_float(r[i]), scale, sum[c + i]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_acc_empty + 8 * acc);
+                if (++acc == kAccs) { acc = 0; ++acc_round; }
+                scale = ahead;
+            }
+            if (!ok) break;
+            RowStore rs;
+            rs.bf16 = p.bf16 != 0;
+            rs.f32 = p.f32 != 0;
+            rs.gate = nullptr;
+            rs.gate_row_bytes = 0;
+            rs.row_bytes = p.out_row_bytes;
+            rs.rows = row0 >= span.end ? 0u : span.end - row0 < 32 ? (uint32_t)(span.end - row0) : 32u;
+            unsigned char* out = p.out + row0 * p.out_row_bytes;
+            if (p.relu) {
+#pragma unroll
+                for (int i = 0; i < kCols; ++i) sum[i] = relu(sum[i]);
+            }
+            const uint32_t cols = col0 >= p.n_out ? 0u : p.n_out - col0 < (uint32_t)kCols ? p.n_out - col0 : (uint32_t)kCols;
+            if (p.f32) {
+#pragma unroll
+                for (int c = 0; c < kCols; c += 32) {
+                    if ((uint32_t)c >= cols) continue;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        stage_unit(stage, lane, u, make_uint4(__float_as_uint(sum[c + 4 * u]), __float_as_uint(sum[c + 4 * u + 1]),
+                                                              __float_as_uint(sum[c + 4 * u + 2]), __float_as_uint(sum[c + 4 * u + 3])));
+                    rs.bytes = (cols - c < 32u ? cols - c : 32u) * 4u;
+                    rs.out = out + (size_t)(col0 + c) * 4;
+                    store_rows(rs, stage);
+                }
+            } else {
+                constexpr int kPer = kCols < 64 ? kCols : 64;
+#pragma unroll
+                for (int c = 0; c < kCols; c += kPer) {
+                    if ((uint32_t)c >= cols) continue;
+#pragma unroll
+                    for (int u = 0; u < kPer / 8; ++u)
+                        stage_unit(stage, lane, u, make_uint4(pack16(sum[c + 8 * u], sum[c + 8 * u + 1], rs.bf16), pack16(sum[c + 8 * u + 2], sum[c + 8 * u + 3], rs.bf16),
+                                                              pack16(sum[c + 8 * u + 4], sum[c + 8 * u + 5], rs.bf16), pack16(sum[c + 8 * u + 6], sum[c + 8 * u + 7], rs.bf16)));
+                    rs.bytes = (cols - c < (uint32_t)kPer ? cols - c : (uint32_t)kPer) * 2u;
+                    rs.out = out + (size_t)(col0 + c) * 2;
+                    store_rows(rs, stage);
+                }
+            }
+        }
+    }
+    if ((bad || (!ok && lane == 0)) && p.error_flags) atomicOr(p.error_flags, (ok ? 0u : 2u) | (bad ? 16u : 0u));
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) tmem_free(tmem, kTmemCols);
+}
+
+template <int BN>
+const char* launch(const CUtensorMap& a, const CUtensorMap& b, const Fp8Args& args, uint64_t max_units, cudaStream_t stream) {
+    static_assert(smem_bytes<BN>() <= 227 * 1024, "shared memory of one SM");
+    const int sms = sm_count();
+    if (cudaFuncSetAttribute((const void*)k_grouped_fp8<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<BN>()) != cudaSuccess)
+        return "cudaFuncSetAttribute failed";
+    const int grid = (int)(max_units < (uint64_t)sms ? max_units : (uint64_t)sms);
+    k_grouped_fp8<BN><<<grid, kThreads, smem_bytes<BN>(), stream>>>(a, b, args);
+    return nullptr;
+}
+
+}  // namespace
+
+const char* launch_grouped_matmul_fp8(const srf_grouped_t& p, const uint64_t* offsets, const void* x, const float* x_scales,
+                                      const void* w, const float* w_scales, void* y, unsigned int* error_flags,
+                                      cudaStream_t stream) {
+    const uint64_t busy = p.n_groups < p.n_rows ? p.n_groups : p.n_rows;
+    const uint64_t row_tiles = p.n_rows / kBM + busy;
+    if (!row_tiles) return nullptr;
+    const uint64_t want = 2ull * sm_count();
+    int bn = 256;
+    while (bn > 64 && ((uint32_t)bn / 2 >= p.n_out || row_tiles * ((p.n_out + bn - 1) / bn) < want)) bn /= 2;
+    CUtensorMap a, b;
+    if (!make_operand_map(&a, x, SRF_TYPE_E4M3, p.n_in, p.n_rows, p.ld_x, 0, 0, kBM) ||
+        !make_operand_map(&b, w, SRF_TYPE_E4M3, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, bn))
+        return "the driver refused an operand's tensor map";
+    Fp8Args k;
+    memset(&k, 0, sizeof(k));
+    k.offsets = offsets; k.out = (unsigned char*)y; k.x_scales = x_scales; k.w_scales = w_scales; k.n_rows = p.n_rows;
+    k.n_groups = p.n_groups; k.n_in = p.n_in; k.n_out = p.n_out;
+    k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.out_type == SRF_TYPE_BF16; k.relu = p.activation == SRF_ACT_RELU;
+    k.out_row_bytes = p.ld_y * (k.f32 ? 4 : 2); k.error_flags = error_flags;
+    const uint64_t units = row_tiles * ((p.n_out + bn - 1) / bn);
+    switch (bn) {
+    case 256: return launch<256>(a, b, k, units, stream);
+    case 128: return launch<128>(a, b, k, units, stream);
+    default: return launch<64>(a, b, k, units, stream);
+    }
+}
+
+}  // namespace srf

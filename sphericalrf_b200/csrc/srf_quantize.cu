@@ -1,0 +1,164 @@
+// srf_quantize.cu -- 16-bit values to e4m3 values and fp32 scales, for srf_grouped_fp8.cu.
+//
+// A block shares one scale s = amax / 448, amax over the block's finite values (1 where that is 0, and at least 2^-126,
+// below which a quotient could leave the range); q = the e4m3 value nearest to v / s, ties to even.  The division is
+// IEEE's: a product with 1/s would move values next to a tie.  Infinities and NaNs become e4m3's NaN and do not touch
+// the block's other values.
+//
+// Bound by memory: two bytes read, one written per value, one pass (the block stays in registers between the maximum
+// and the quotients).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "srf_layers.cuh"
+
+namespace srf {
+
+namespace {
+
+constexpr float kE4m3Max = 448.f;
+constexpr float kScaleMin = 1.17549435e-38f;      // 2^-126
+
+__device__ __forceinline__ void unpack8(uint4 v, bool bf16, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (bf16) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+            const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[2 * i] = t.x;
+            f[2 * i + 1] = t.y;
+        }
+    }
+}
+
+// Eight values from `p`, of which `have` (0..8) exist; zeros behind them.
+__device__ __forceinline__ uint4 load8(const uint16_t* p, int have) {
+    if (have >= 8) return __ldg(reinterpret_cast<const uint4*>(p));
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < have) w[i >> 1] |= (uint32_t)__ldg(p + i) << ((i & 1) * 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __int_as_float(0x7f800000); }
+
+__device__ __forceinline__ float amax8(const float (&f)[8], float top) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = finite(f[i]) ? fmaxf(top, fabsf(f[i])) : top;
+    return top;
+}
+
+__device__ __forceinline__ float scale_of(float amax) { return amax > 0.f ? fmaxf(amax / kE4m3Max, kScaleMin) : 1.f; }
+
+__device__ __forceinline__ uint2 quantize8(const float (&f)[8], float scale) {
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float nan = __int_as_float(0x7fffffff);
+        const float lo = finite(f[2 * i]) ? f[2 * i] / scale : nan, hi = finite(f[2 * i + 1]) ? f[2 * i + 1] / scale : nan;
+        uint16_t t;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(t) : "f"(hi), "f"(lo));
+        h[i] = t;
+    }
+    return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+}
+
+__device__ __forceinline__ void store8(unsigned char* p, int have, uint2 v) {
+    if (have >= 8) { *reinterpret_cast<uint2*>(p) = v; return; }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < have) p[i] = (unsigned char)((i < 4 ? v.x >> (8 * i) : v.y >> (8 * (i - 4))) & 255u);
+}
+
+// Rows x 128: half a warp holds one block of one row (eight values a lane); a warp takes two neighbouring blocks of
+// four rows, so that four loads of 16 bytes per lane are in flight.
+constexpr int kRowsPerWarp = 4;
+
+__global__ void __launch_bounds__(256)
+k_quantize_rows(int bf16, uint64_t n_rows, const uint64_t* __restrict__ n_used, uint32_t n_cols, const uint16_t* __restrict__ in,
+                uint64_t ld_in, unsigned char* __restrict__ out, uint64_t ld_out, float* __restrict__ scales) {
+    uint64_t rows = n_rows;
+    if (n_used) { const uint64_t u = __ldg((const unsigned long long*)n_used); rows = u < rows ? u : rows; }
+    const int lane = threadIdx.x & 31;
+    const uint32_t block = blockIdx.y * 2 + (lane >> 4);
+    const uint64_t row0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * kRowsPerWarp;
+    if (row0 >= rows) return;
+    const uint32_t col = block * 128 + (lane & 15) * 8;
+    const int have = col >= n_cols ? 0 : n_cols - col < 8 ? (int)(n_cols - col) : 8;
+    uint4 v[kRowsPerWarp];
+#pragma unroll
+    for (int i = 0; i < kRowsPerWarp; ++i) v[i] = row0 + i < rows ? load8(in + (row0 + i) * ld_in + col, have) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int i = 0; i < kRowsPerWarp; ++i) {
+        float f[8];
+        unpack8(v[i], bf16 != 0, f);
+        float top = amax8(f, 0.f);
+#pragma unroll
+        for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float scale = scale_of(top);
+        if (row0 + i < rows) {
+            if (have > 0) store8(out + (row0 + i) * ld_out + col, have, quantize8(f, scale));
+            if ((lane & 15) == 0 && block * 128 < n_cols) scales[(uint64_t)block * n_rows + row0 + i] = scale;
+        }
+    }
+}
+
+// 128 x 128: a CTA holds one block, 64 values a thread.
+__global__ void __launch_bounds__(256)
+k_quantize_weights(int bf16, uint32_t n_rows, uint32_t n_cols, const uint16_t* __restrict__ in, uint64_t ld_in, uint64_t stride_in,
+                   unsigned char* __restrict__ out, uint64_t ld_out, uint64_t stride_out, float* __restrict__ scales) {
+    const uint32_t bx = blockIdx.x, by = blockIdx.y, mat = blockIdx.z;
+    const uint32_t col = bx * 128 + (threadIdx.x & 15) * 8, row0 = by * 128 + (threadIdx.x >> 4);
+    const int have = col >= n_cols ? 0 : n_cols - col < 8 ? (int)(n_cols - col) : 8;
+    in += mat * stride_in;
+    out += mat * stride_out;
+    uint4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = row0 + 16 * i < n_rows ? load8(in + (uint64_t)(row0 + 16 * i) * ld_in + col, have) : make_uint4(0u, 0u, 0u, 0u);
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float f[8];
+        unpack8(v[i], bf16 != 0, f);
+        top = amax8(f, top);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    __shared__ float sh[8];
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, sh[i]);
+    const float scale = scale_of(top);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (row0 + 16 * i < n_rows && have > 0) {
+            float f[8];
+            unpack8(v[i], bf16 != 0, f);
+            store8(out + (uint64_t)(row0 + 16 * i) * ld_out + col, have, quantize8(f, scale));
+        }
+    }
+    if (threadIdx.x == 0) scales[((uint64_t)mat * gridDim.y + by) * gridDim.x + bx] = scale;
+}
+
+}  // namespace
+
+void launch_quantize_rows(int type, uint64_t n_rows, const uint64_t* n_rows_used, uint32_t n_cols, const void* in, uint64_t ld_in,
+                          void* out, uint64_t ld_out, float* scales, cudaStream_t stream) {
+    if (!n_rows) return;
+    const dim3 grid((uint32_t)((n_rows + 8 * kRowsPerWarp - 1) / (8 * kRowsPerWarp)), (n_cols + 255) / 256);
+    k_quantize_rows<<<grid, 256, 0, stream>>>(type == SRF_TYPE_BF16, n_rows, n_rows_used, n_cols, (const uint16_t*)in, ld_in,
+                                              (unsigned char*)out, ld_out, scales);
+}
+
+void launch_quantize_weights(int type, uint32_t n_matrices, uint32_t n_rows, uint32_t n_cols, const void* in, uint64_t ld_in,
+                             uint64_t stride_in, void* out, uint64_t ld_out, uint64_t stride_out, float* scales, cudaStream_t stream) {
+    const dim3 grid((n_cols + 127) / 128, (n_rows + 127) / 128, n_matrices);
+    k_quantize_weights<<<grid, 256, 0, stream>>>(type == SRF_TYPE_BF16, n_rows, n_cols, (const uint16_t*)in, ld_in, stride_in,
+                                                 (unsigned char*)out, ld_out, stride_out, scales);
+}
+
+}  // namespace srf
