@@ -30,11 +30,11 @@ namespace {
 
 enum Mode { kLayer = 0, kInputGrad = 1, kWeightGrad = 2 };
 
-constexpr int kThreads = 256;                 // TMA, MMA, TMEM owner, spare, 4 epilogue warps
+constexpr int kThreads = 384;                 // TMA, MMA, TMEM owner, spare, two sets of 4 epilogue warps
 constexpr int kBM = 128, kBK = 64;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kABytes = kBM * kBK * 2;
-constexpr int kStoreBytes = 4 * 4096;         // staging of the four epilogue warps
+constexpr int kStoreBytes = 8 * 4096;         // staging of the epilogue warps
 constexpr int kSmemMin = 120 * 1024;          // a second CTA that allocates TMEM must never share the SM
 
 struct GroupedArgs {
@@ -42,9 +42,8 @@ struct GroupedArgs {
     unsigned char* out;
     const unsigned char* gate;
     float* partial;               // weight gradient: two tiles of partial sums per CTA
-    uint64_t n_rows;
     uint64_t out_row_bytes, out_group_bytes, gate_row_bytes;
-    uint32_t n_groups;
+    uint32_t n_rows, n_groups;
     uint32_t out_rows;            // weight gradient: n_out
     uint32_t out_cols;            // n_out, n_in, n_in
     uint32_t depth;               // summed length of the first two products
@@ -55,6 +54,8 @@ struct GroupedArgs {
 template <int BN>
 __host__ __device__ constexpr int n_stages() { return BN == 256 ? 4 : BN == 128 ? 6 : 8; }
 template <int BN>
+__host__ __device__ constexpr int n_accs() { return BN == 256 ? 2 : 4; }
+template <int BN>
 __host__ __device__ constexpr int smem_bytes() {
     const int b = 1024 + n_stages<BN>() * (kABytes + BN * kBK * 2) + kStoreBytes + 512;
     return b < kSmemMin ? kSmemMin : b;
@@ -63,8 +64,8 @@ __host__ __device__ constexpr int smem_bytes() {
 // Units of work of a group: whole output tiles for the first two products; 64-sample stages of output tiles for the
 // weight gradient, whose work is cut evenly across the CTAs (see below).
 template <int MODE>
-__device__ __forceinline__ uint64_t group_units(const Span& s, uint32_t tiles_across) {
-    const uint64_t rows = s.end - s.begin;
+__device__ __forceinline__ uint32_t group_units(const Span& s, uint32_t tiles_across) {
+    const uint32_t rows = s.end - s.begin;
     return (MODE == kWeightGrad ? (rows + kBK - 1) / kBK : (rows + kBM - 1) / kBM) * tiles_across;
 }
 
@@ -72,10 +73,10 @@ __device__ __forceinline__ uint64_t group_units(const Span& s, uint32_t tiles_ac
 struct Piece {
     uint32_t group;
     Span span;
-    uint64_t m;            // first output row: sample (first two products) or row of W (weight gradient)
+    uint32_t m;            // first output row: sample (first two products) or row of W (weight gradient)
     uint32_t n;            // output column tile
-    uint64_t k0;           // first stage
-    uint64_t k_stages;     // stages
+    uint32_t k0;           // first stage
+    uint32_t k_stages;     // stages
     bool whole;            // the piece is the tile's whole sum
     bool first;            // the piece holds the tile's first stage
 };
@@ -85,32 +86,39 @@ struct Piece {
 // Weight gradient: the stages of all tiles are one line of `units` which the CTAs share out evenly, so ragged groups
 // balance by themselves and a narrow layer (one tile per group) still fills every SM.  A tile that a boundary cuts
 // is summed from the CTAs' partial sums, in the CTAs' order, by a second kernel: the same result on every run.
+__device__ __forceinline__ uint32_t first_unit(uint32_t units, uint32_t cta, uint32_t n_ctas) {
+    const uint32_t q = units / n_ctas, r = units - q * n_ctas;
+    return cta * q + (cta < r ? cta : r);
+}
+
 template <int MODE>
 struct Pieces {
     GroupWalk walk;
-    uint64_t at, stop;
-    __device__ __forceinline__ void init(uint64_t units) {
+    uint32_t at, stop, step;
+    // first two products: pieces start, start + step, ... of those dealt to this CTA
+    __device__ __forceinline__ void init(uint32_t units, uint32_t start, uint32_t every) {
         if (MODE == kWeightGrad) {
-            const uint64_t q = units / gridDim.x, r = units % gridDim.x;
-            at = blockIdx.x * q + (blockIdx.x < r ? blockIdx.x : r);
-            stop = at + q + (blockIdx.x < r ? 1 : 0);
+            at = first_unit(units, blockIdx.x, gridDim.x);
+            stop = first_unit(units, blockIdx.x + 1, gridDim.x);
+            step = 0;
         } else {
-            at = blockIdx.x;
-            stop = ~0ull;
+            at = blockIdx.x + start * gridDim.x;
+            stop = 0xffffffffu;
+            step = every * gridDim.x;
         }
     }
     __device__ __forceinline__ bool next(const GroupedArgs& p, uint32_t tiles_m, uint32_t tiles_n, Piece* o, bool* bad) {
         if (at >= stop) return false;
         const uint32_t across = MODE == kWeightGrad ? tiles_m * tiles_n : tiles_n;
-        uint64_t local;
+        uint32_t local;
         if (!walk.find(at, p.offsets, p.n_groups, p.n_rows, [&](const Span& s) { return group_units<MODE>(s, across); },
                        &o->group, &o->span, &local, bad))
             return false;
-        const uint64_t rows = o->span.end - o->span.begin;
+        const uint32_t rows = o->span.end - o->span.begin;
+        uint32_t m;
         if (MODE == kWeightGrad) {
-            const uint64_t deep = (rows + kBK - 1) / kBK;
-            const uint64_t t = local / deep;
-            uint64_t m;
+            const uint32_t deep = (rows + kBK - 1) / kBK;
+            const uint32_t t = local / deep;
             tile_place(t, tiles_m, tiles_n, &m, &o->n);
             o->m = m * kBM;
             o->k0 = local - t * deep;
@@ -119,13 +127,12 @@ struct Pieces {
             o->whole = o->k_stages == deep;
             at += o->k_stages;
         } else {
-            uint64_t m;
             tile_place(local, (rows + kBM - 1) / kBM, tiles_n, &m, &o->n);
             o->m = o->span.begin + m * kBM;
             o->k0 = 0;
             o->k_stages = (p.depth + kBK - 1) / kBK;
             o->first = o->whole = true;
-            at += gridDim.x;
+            at += step;
         }
         return true;
     }
@@ -133,8 +140,8 @@ struct Pieces {
 
 // Units of all groups (warp-collective).
 template <int MODE>
-__device__ __forceinline__ uint64_t all_units(const GroupedArgs& p, uint32_t across, bool* bad) {
-    uint64_t sum = 0;
+__device__ __forceinline__ uint32_t all_units(const GroupedArgs& p, uint32_t across, bool* bad) {
+    uint32_t sum = 0;
     for (uint32_t g = threadIdx.x & 31; g < p.n_groups; g += 32) sum += group_units<MODE>(group_span(p.offsets, g, p.n_rows, bad), across);
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -144,7 +151,7 @@ __device__ __forceinline__ uint64_t all_units(const GroupedArgs& p, uint32_t acr
 template <int MODE, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
 k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GroupedArgs p) {
-    constexpr int kStages = n_stages<BN>();
+    constexpr int kStages = n_stages<BN>(), kAccs = n_accs<BN>();
     constexpr int kBBytes = BN * kBK * 2;
     constexpr bool kAColumns = MODE == kWeightGrad, kBColumns = MODE != kLayer;     // read down the columns: MN-major
     extern __shared__ unsigned char smem_raw[];
@@ -153,17 +160,17 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     unsigned char* sm_b = smem + kStages * kABytes;
     unsigned char* sm_store = sm_b + kStages * kBBytes;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm_store + kStoreBytes);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2 * kAccs);
     volatile uint32_t* failed = tmem_slot + 1;
     const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kStages;
-    const uint32_t bar_acc_full = bar_empty + 8 * kStages, bar_acc_empty = bar_acc_full + 16;
+    const uint32_t bar_acc_full = bar_empty + 8 * kStages, bar_acc_empty = bar_acc_full + 8 * kAccs;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t tiles_n = (p.out_cols + BN - 1) / BN;
     const uint32_t tiles_m = MODE == kWeightGrad ? (p.out_rows + kBM - 1) / kBM : 0;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(bar_acc_full + 8 * i, 1); mbar_init(bar_acc_empty + 8 * i, 4); }
+        for (int i = 0; i < kAccs; ++i) { mbar_init(bar_acc_full + 8 * i, 1); mbar_init(bar_acc_empty + 8 * i, 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *failed = 0;
         tma_prefetch_map(&map_a);
@@ -177,7 +184,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 
     bool bad = false, ok = true;
     Pieces<MODE> pieces;
-    pieces.init(MODE == kWeightGrad ? all_units<MODE>(p, tiles_m * tiles_n, &bad) : 0);
+    const bool storing = MODE != kWeightGrad && warp >= 4;       // the two sets of epilogue warps take every other piece
+    pieces.init(MODE == kWeightGrad ? all_units<MODE>(p, tiles_m * tiles_n, &bad) : 0, storing ? (warp - 4) >> 2 : 0, storing ? 2 : 1);
     Piece t;
 
     if (warp == 0) {
@@ -185,7 +193,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         uint32_t s = 0, round = 0;                     // ring position
         uint32_t in_flight = 0;
         while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
-            for (uint64_t k = 0; k < t.k_stages; ++k) {
+            for (uint32_t k = 0; k < t.k_stages; ++k) {
                 if (round > 0 && !mbar_wait(bar_empty + 8 * s, (round - 1) & 1, failed)) { ok = false; break; }
                 if (elect_one()) {
                     const uint32_t bar = bar_full + 8 * s, a = smem_u32(sm_a) + s * kABytes, b = smem_u32(sm_b) + s * kBBytes;
@@ -228,14 +236,14 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
             if (acc_round > 0 && !mbar_wait(bar_acc_empty + 8 * acc, (acc_round - 1) & 1, failed)) { ok = false; break; }
             tc_fence_after();
-            const uint32_t d = tmem + acc * 256;
-            for (uint64_t k = 0; k < t.k_stages; ++k) {
+            const uint32_t d = tmem + acc * BN;
+            for (uint32_t k = 0; k < t.k_stages; ++k) {
                 if (!mbar_wait(bar_full + 8 * s, round & 1, failed)) { ok = false; break; }
                 tc_fence_after();
                 int k_steps = kBK / 16;
                 if (MODE == kWeightGrad) {
-                    const uint64_t left = t.span.end - t.span.begin - (t.k0 + k) * kBK;     // samples of this stage
-                    if (left < (uint64_t)kBK) {
+                    const uint32_t left = t.span.end - t.span.begin - (t.k0 + k) * kBK;     // samples of this stage
+                    if (left < (uint32_t)kBK) {
                         // the group's last stage: instructions cover whole 16s, so zero up to the next 16
                         const int r0 = (int)left, r1 = (r0 + 15) & ~15;
                         k_steps = r1 / 16;
@@ -254,7 +262,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     for (int q = 0; q < k_steps; ++q) {
                         const uint64_t da = kAColumns ? operand_desc(a + q * 2048, 8192, 1024) : operand_desc(a + q * 32, 16, 1024);
                         const uint64_t db = kBColumns ? operand_desc(b + q * 2048, 8192, 1024) : operand_desc(b + q * 32, 16, 1024);
-                        mma_f16(d, da, db, idesc, (k | (uint64_t)q) != 0);
+                        mma_f16(d, da, db, idesc, (k | (uint32_t)q) != 0);
                     }
                     mma_commit(bar_empty + 8 * s);
                     if (k + 1 == t.k_stages) mma_commit(bar_acc_full + 8 * acc);
@@ -263,26 +271,25 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 if (++s == kStages) { s = 0; ++round; }
             }
             if (!ok) break;
-            if (++acc == 2) { acc = 0; ++acc_round; }
+            if (++acc == kAccs) { acc = 0; ++acc_round; }
         }
     } else if (warp >= 4) {
         // ---- finished accumulators to memory ----
-        const int quarter = warp & 3;
-        unsigned char* stage = sm_store + quarter * 4096;
-        uint32_t acc = 0, acc_round = 0;
+        const int quarter = warp & 3, set = (warp - 4) >> 2;
+        unsigned char* stage = sm_store + (warp - 4) * 4096;
+        uint32_t acc = set, acc_round = 0;
+        if (MODE == kWeightGrad && set) pieces.next(p, tiles_m, tiles_n, &t, &bad);
         while (pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
-            if (!mbar_wait(bar_acc_full + 8 * acc, acc_round & 1, failed)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t d = tmem + acc * 256 + ((uint32_t)(quarter * 32) << 16);
             RowStore rs;
             rs.bf16 = p.bf16 != 0;
             rs.gate = nullptr;
             rs.gate_row_bytes = p.gate_row_bytes;
             const bool partial = MODE == kWeightGrad && !t.whole;
+            const bool gated = MODE == kInputGrad && p.gate;
             rs.f32 = partial || p.f32;
-            const uint64_t row0 = t.m + (uint64_t)quarter * 32;
-            const uint64_t end = MODE == kWeightGrad ? (uint64_t)p.out_rows : t.span.end;
-            rs.rows = row0 >= end ? 0u : end - row0 < 32 ? (uint32_t)(end - row0) : 32u;
+            const uint32_t row0 = t.m + quarter * 32;
+            const uint32_t end = MODE == kWeightGrad ? p.out_rows : t.span.end;
+            rs.rows = row0 >= end ? 0u : end - row0 < 32 ? end - row0 : 32u;
             const uint32_t col0 = t.n * BN;
             const uint32_t cols = p.out_cols - col0 < (uint32_t)BN ? p.out_cols - col0 : (uint32_t)BN;
             unsigned char* out;
@@ -294,7 +301,18 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 out = p.out + (MODE == kWeightGrad ? t.group * p.out_group_bytes : 0ull) + row0 * p.out_row_bytes;
                 rs.row_bytes = p.out_row_bytes;
             }
-            const uint32_t per = rs.f32 ? 32u : 64u;
+            const uint32_t per = rs.f32 ? 32u : 64u, size = rs.f32 ? 4u : 2u;
+            auto piece = [&](uint32_t c) {
+                rs.bytes = (cols - c < per ? cols - c : per) * size;
+                rs.out = out + (size_t)(partial ? c : col0 + c) * size;
+                if (gated) rs.gate = p.gate + row0 * p.gate_row_bytes + (size_t)(col0 + c) * 2;
+            };
+            uint4 hv[8];
+            piece(0);
+            if (gated) load_gate(rs, hv);                  // on its way while the sums finish
+            if (!mbar_wait(bar_acc_full + 8 * acc, acc_round & 1, failed)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
             for (uint32_t c = 0; c < cols; c += per) {
                 uint32_t r[32];
                 if (rs.f32) {
@@ -322,18 +340,25 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         }
                     }
                 }
-                if (c + per >= cols) {             // the accumulator is read: the next tile may have it
+                if (c + per >= cols) {             // the accumulator is read: a later tile may have it
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar_acc_empty + 8 * acc);
                 }
-                const uint32_t size = rs.f32 ? 4u : 2u;
-                rs.bytes = (cols - c < per ? cols - c : per) * size;
-                rs.out = out + (size_t)(partial ? c : col0 + c) * size;
-                if (MODE == kInputGrad && p.gate) rs.gate = p.gate + row0 * p.gate_row_bytes + (size_t)(col0 + c) * 2;
-                store_rows(rs, stage);
+                if (gated) {
+                    store_rows<true>(rs, stage, hv);
+                    if (c + per < cols) {
+                        piece(c + per);
+                        load_gate(rs, hv);
+                    }
+                } else {
+                    store_rows(rs, stage);
+                    piece(c + per);
+                }
             }
-            if (++acc == 2) { acc = 0; ++acc_round; }
+            acc += 2;
+            if (acc >= kAccs) { acc -= kAccs; ++acc_round; }
+            if (MODE == kWeightGrad && !pieces.next(p, tiles_m, tiles_n, &t, &bad)) break;     // the other set's piece
         }
     }
     if ((bad || (!ok && lane == 0)) && p.error_flags) atomicOr(p.error_flags, (ok ? 0u : 2u) | (bad ? 16u : 0u));
@@ -342,58 +367,74 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if (warp == 2) tmem_free(tmem, kTmemCols);
 }
 
-// Second kernel of the weight gradient.  Block (tile, group, slice of 16 rows): sums the partial tiles of an output
-// tile that more than one CTA worked on, in the CTAs' order, or writes the zeros of a group without samples.
+// Second kernel of the weight gradient.  Blocks (c, slice) with c < n_ctas - 1: the boundary behind CTA c.  If it cuts an
+// output tile and is the first to cut it, sums the tile's partial sums in the CTAs' order (the slice: a few of its rows).
+// The other blocks (n_ctas - 1 + g, slice) write the zeros of a group without samples.
+constexpr int kJoinSlices = 16, kJoinThreads = 256;
+
 template <int BN>
-__global__ void __launch_bounds__(256) k_weight_grad_join(const GroupedArgs p, uint32_t n_ctas) {
+__global__ void __launch_bounds__(kJoinThreads) k_weight_grad_join(const GroupedArgs p, uint32_t n_ctas) {
     const uint32_t tiles_n = (p.out_cols + BN - 1) / BN, tiles_m = (p.out_rows + kBM - 1) / kBM;
-    const uint32_t across = tiles_m * tiles_n;
-    const uint32_t g = blockIdx.y, tile_id = blockIdx.x / (kBM / 16), slice = blockIdx.x % (kBM / 16);
-    __shared__ uint64_t sh_units[2];
+    const uint32_t across = tiles_m * tiles_n, slice = blockIdx.y;
     bool bad = false;
+    if (blockIdx.x >= n_ctas - 1) {
+        const uint32_t g = blockIdx.x - (n_ctas - 1);
+        const Span s = group_span(p.offsets, g, p.n_rows, &bad);
+        if (s.end > s.begin) return;
+        for (uint32_t row = slice; row < p.out_rows; row += kJoinSlices) {
+            unsigned char* o = p.out + g * p.out_group_bytes + row * p.out_row_bytes;
+            for (uint32_t col = threadIdx.x; col < p.out_cols; col += kJoinThreads) {
+                if (p.f32) reinterpret_cast<float*>(o)[col] = 0.f;
+                else reinterpret_cast<uint16_t*>(o)[col] = 0;
+            }
+        }
+        return;
+    }
+    __shared__ uint32_t sh[5];         // first and last CTA of the tile, its group, m, n
     if (threadIdx.x < 32) {
-        uint64_t all = 0, before = 0;
-        for (uint32_t q = threadIdx.x; q < p.n_groups; q += 32) {
-            const uint64_t u = group_units<kWeightGrad>(group_span(p.offsets, q, p.n_rows, &bad), across);
-            all += u;
-            if (q < g) before += u;
+        const uint32_t units = all_units<kWeightGrad>(p, across, &bad);
+        const uint32_t u = first_unit(units, blockIdx.x + 1, n_ctas);       // first unit behind the boundary
+        GroupWalk walk;
+        uint32_t group = 0, local = 0, c0 = 1, c1 = 0, m = 0, n = 0;
+        Span s = {0, 0};
+        if (u > 0 && u < units &&
+            walk.find(u, p.offsets, p.n_groups, p.n_rows, [&](const Span& q) { return group_units<kWeightGrad>(q, across); }, &group, &s, &local, &bad)) {
+            const uint32_t deep = (s.end - s.begin + kBK - 1) / kBK, t = local / deep, k = local - t * deep;
+            const uint32_t u0 = u - k, before = first_unit(units, blockIdx.x, n_ctas);
+            // the boundary cuts the tile, and the one in front of it does not
+            if (k > 0 && before <= u0 && before < u) {
+                c0 = blockIdx.x;
+                c1 = c0 + 1;
+                while (c1 + 1 < n_ctas && first_unit(units, c1 + 1, n_ctas) < u0 + deep) ++c1;
+                tile_place(t, tiles_m, tiles_n, &m, &n);
+            }
         }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) {
-            all += __shfl_xor_sync(0xffffffffu, all, d);
-            before += __shfl_xor_sync(0xffffffffu, before, d);
-        }
-        if (threadIdx.x == 0) { sh_units[0] = all; sh_units[1] = before; }
+        if (threadIdx.x == 0) { sh[0] = c0; sh[1] = c1; sh[2] = group; sh[3] = m; sh[4] = n; }
     }
     __syncthreads();
-    const Span s = group_span(p.offsets, g, p.n_rows, &bad);
-    const uint64_t deep = (s.end - s.begin + kBK - 1) / kBK;
-    uint32_t c0 = 0, c1 = 0;
-    if (deep) {
-        // CTA c works on units [c q + min(c, r), ...): the owners of the tile's first and last unit
-        const uint64_t q = sh_units[0] / n_ctas, r = sh_units[0] % n_ctas;
-        const uint64_t u0 = sh_units[1] + tile_id * deep, u1 = u0 + deep - 1;
-        auto owner = [&](uint64_t u) { return (uint32_t)(u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q); };
-        c0 = owner(u0);
-        c1 = owner(u1);
-        if (c0 == c1) return;
-    }
-    uint64_t m;
-    uint32_t n;
-    tile_place(tile_id, tiles_m, tiles_n, &m, &n);
-    for (uint32_t i = threadIdx.x; i < 16 * BN; i += blockDim.x) {
-        const uint32_t row = slice * 16 + i / BN, col = i % BN;
-        const uint64_t orow = m * kBM + row;
-        const uint32_t ocol = n * BN + col;
+    const uint32_t c0 = sh[0], c1 = sh[1];
+    if (c0 > c1) return;
+    constexpr uint32_t kRows = kBM / kJoinSlices, kQuads = kRows * BN / 4;
+    for (uint32_t i = threadIdx.x; i < kQuads; i += kJoinThreads) {
+        const uint32_t row = slice * kRows + i / (BN / 4), col = i % (BN / 4) * 4;
+        const uint32_t orow = sh[3] * kBM + row, ocol = sh[4] * BN + col;
         if (orow >= p.out_rows || ocol >= p.out_cols) continue;
-        float sum = 0.f;
-        if (deep) {
-            sum = p.partial[((size_t)c0 * 2 + 1) * kBM * BN + (size_t)row * BN + col];
-            for (uint32_t c = c0 + 1; c <= c1; ++c) sum += p.partial[(size_t)c * 2 * kBM * BN + (size_t)row * BN + col];
+        const float4* q = reinterpret_cast<const float4*>(p.partial + (size_t)row * BN + col);
+        constexpr size_t kSlot = (size_t)kBM * BN / 4;
+        float4 sum = q[(2 * (size_t)c0 + 1) * kSlot];
+#pragma unroll 8
+        for (uint32_t c = c0 + 1; c <= c1; ++c) {
+            const float4 v = q[2 * (size_t)c * kSlot];
+            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
         }
-        unsigned char* o = p.out + g * p.out_group_bytes + orow * p.out_row_bytes;
-        if (p.f32) reinterpret_cast<float*>(o)[ocol] = sum;
-        else reinterpret_cast<uint16_t*>(o)[ocol] = (uint16_t)pack16(sum, 0.f, p.bf16 != 0);
+        unsigned char* o = p.out + sh[2] * p.out_group_bytes + orow * p.out_row_bytes;
+        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (ocol + e >= p.out_cols) continue;
+            if (p.f32) reinterpret_cast<float*>(o)[ocol + e] = f[e];
+            else reinterpret_cast<uint16_t*>(o)[ocol + e] = (uint16_t)pack16(f[e], 0.f, p.bf16 != 0);
+        }
     }
 }
 
@@ -468,7 +509,7 @@ const char* launch_grouped_matmul(const srf_grouped_t& p, const uint64_t* offset
         return "the driver refused an operand's tensor map";
     GroupedArgs k;
     memset(&k, 0, sizeof(k));
-    k.offsets = offsets; k.out = (unsigned char*)y; k.n_rows = p.n_rows; k.n_groups = p.n_groups;
+    k.offsets = offsets; k.out = (unsigned char*)y; k.n_rows = (uint32_t)p.n_rows; k.n_groups = p.n_groups;
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16; k.relu = p.activation == SRF_ACT_RELU;
     k.out_row_bytes = p.ld_y * (k.f32 ? 4 : 2); k.out_cols = p.n_out; k.depth = p.n_in; k.error_flags = error_flags;
     const uint64_t units = row_tiles * ((p.n_out + bn - 1) / bn);
@@ -491,7 +532,7 @@ const char* launch_grouped_input_grad(const srf_grouped_t& p, const uint64_t* of
         return "the driver refused an operand's tensor map";
     GroupedArgs k;
     memset(&k, 0, sizeof(k));
-    k.offsets = offsets; k.out = (unsigned char*)dx; k.gate = (const unsigned char*)gate; k.n_rows = p.n_rows; k.n_groups = p.n_groups;
+    k.offsets = offsets; k.out = (unsigned char*)dx; k.gate = (const unsigned char*)gate; k.n_rows = (uint32_t)p.n_rows; k.n_groups = p.n_groups;
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16;
     k.out_row_bytes = p.ld_x * (k.f32 ? 4 : 2); k.gate_row_bytes = p.ld_x * 2; k.out_cols = p.n_in; k.depth = p.n_out;
     k.error_flags = error_flags;
@@ -512,7 +553,7 @@ const char* launch_grouped_weight_grad(const srf_grouped_t& p, const uint64_t* o
     const int bn = weight_grad_bn(p);
     GroupedArgs k;
     memset(&k, 0, sizeof(k));
-    k.offsets = offsets; k.out = (unsigned char*)dw; k.partial = (float*)workspace; k.n_rows = p.n_rows; k.n_groups = p.n_groups;
+    k.offsets = offsets; k.out = (unsigned char*)dw; k.partial = (float*)workspace; k.n_rows = (uint32_t)p.n_rows; k.n_groups = p.n_groups;
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16;
     k.out_row_bytes = p.ld_w * (k.f32 ? 4 : 2); k.out_group_bytes = p.group_stride * (k.f32 ? 4 : 2);
     k.out_rows = p.n_out; k.out_cols = p.n_in; k.error_flags = error_flags;
@@ -531,11 +572,11 @@ const char* launch_grouped_weight_grad(const srf_grouped_t& p, const uint64_t* o
                                     : launch<kWeightGrad, 64>(a, b, k, units, stream);
         if (why) return why;
     }
-    const dim3 join_grid((uint32_t)(across * (kBM / 16)), p.n_groups);
     const uint32_t n_ctas = grid ? grid : 1;
-    if (bn == 256) k_weight_grad_join<256><<<join_grid, 256, 0, stream>>>(k, n_ctas);
-    else if (bn == 128) k_weight_grad_join<128><<<join_grid, 256, 0, stream>>>(k, n_ctas);
-    else k_weight_grad_join<64><<<join_grid, 256, 0, stream>>>(k, n_ctas);
+    const dim3 join_grid(n_ctas - 1 + p.n_groups, kJoinSlices);
+    if (bn == 256) k_weight_grad_join<256><<<join_grid, kJoinThreads, 0, stream>>>(k, n_ctas);
+    else if (bn == 128) k_weight_grad_join<128><<<join_grid, kJoinThreads, 0, stream>>>(k, n_ctas);
+    else k_weight_grad_join<64><<<join_grid, kJoinThreads, 0, stream>>>(k, n_ctas);
     return nullptr;
 }
 

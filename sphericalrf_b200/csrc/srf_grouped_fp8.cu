@@ -28,13 +28,13 @@ struct Fp8Args {
     unsigned char* out;
     const float* x_scales;        // [blocks of n_in][n_rows]
     const float* w_scales;        // [group][blocks of n_out][blocks of n_in]
-    uint64_t n_rows, out_row_bytes;
-    uint32_t n_groups, n_in, n_out;
+    uint64_t out_row_bytes;
+    uint32_t n_rows, n_groups, n_in, n_out;
     int bf16, f32, relu;
     unsigned int* error_flags;
 };
 
-template <int BN> __host__ __device__ constexpr int n_stages() { return BN == 256 ? 3 : BN == 128 ? 5 : 6; }
+template <int BN> __host__ __device__ constexpr int n_stages() { return BN == 256 ? 4 : BN == 128 ? 6 : 8; }
 template <int BN> __host__ __device__ constexpr int n_accs() { return BN == 256 ? 2 : 4; }
 template <int BN>
 __host__ __device__ constexpr int smem_bytes() {
@@ -78,12 +78,10 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 
     bool bad = false, ok = true;
     GroupWalk walk;
-    uint64_t at = blockIdx.x;
-    uint32_t group = 0, tn = 0;
-    uint64_t m = 0;
+    uint32_t at = blockIdx.x, group = 0, tn = 0, m = 0;
     Span span = {0, 0};
     auto next_tile = [&]() -> bool {
-        uint64_t local;
+        uint32_t local;
         if (!walk.find(at, p.offsets, p.n_groups, p.n_rows,
                        [&](const Span& s) { return (s.end - s.begin + kBM - 1) / kBM * tiles_n; }, &group, &span, &local, &bad))
             return false;
@@ -147,8 +145,8 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         unsigned char* stage = sm_store + (warp - 4) * 4096;
         uint32_t acc = 0, acc_round = 0;
         while (ok && next_tile()) {
-            const uint64_t row0 = m + (uint64_t)quarter * 32;
-            const uint64_t row = row0 + lane < p.n_rows ? row0 + lane : p.n_rows - 1;
+            const uint32_t row0 = m + quarter * 32;
+            const uint32_t row = row0 + lane < p.n_rows ? row0 + lane : p.n_rows - 1;
             const uint32_t col0 = tn * BN + half * kCols;
             const uint32_t wb = col0 / 128 < blocks_n ? col0 / 128 : blocks_n - 1;
             const float* sx = p.x_scales + row;
@@ -184,7 +182,7 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             rs.gate = nullptr;
             rs.gate_row_bytes = 0;
             rs.row_bytes = p.out_row_bytes;
-            rs.rows = row0 >= span.end ? 0u : span.end - row0 < 32 ? (uint32_t)(span.end - row0) : 32u;
+            rs.rows = row0 >= span.end ? 0u : span.end - row0 < 32 ? span.end - row0 : 32u;
             unsigned char* out = p.out + row0 * p.out_row_bytes;
             if (p.relu) {
 #pragma unroll
@@ -253,7 +251,7 @@ const char* launch_grouped_matmul_fp8(const srf_grouped_t& p, const uint64_t* of
         return "the driver refused an operand's tensor map";
     Fp8Args k;
     memset(&k, 0, sizeof(k));
-    k.offsets = offsets; k.out = (unsigned char*)y; k.x_scales = x_scales; k.w_scales = w_scales; k.n_rows = p.n_rows;
+    k.offsets = offsets; k.out = (unsigned char*)y; k.x_scales = x_scales; k.w_scales = w_scales; k.n_rows = (uint32_t)p.n_rows;
     k.n_groups = p.n_groups; k.n_in = p.n_in; k.n_out = p.n_out;
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.out_type == SRF_TYPE_BF16; k.relu = p.activation == SRF_ACT_RELU;
     k.out_row_bytes = p.ld_y * (k.f32 ? 4 : 2); k.error_flags = error_flags;

@@ -1,9 +1,16 @@
 // srf_quantize.cu -- 16-bit values to e4m3 values and fp32 scales, for srf_grouped_fp8.cu.
 //
 // A block shares one scale s = amax / 448, amax over the block's finite values (1 where that is 0, and at least 2^-126,
-// below which a quotient could leave the range); q = the e4m3 value nearest to v / s, ties to even.  The division is
-// IEEE's: a product with 1/s would move values next to a tie.  Infinities and NaNs become e4m3's NaN and do not touch
-// the block's other values.
+// below which a quotient could leave the range); q = the e4m3 value nearest to v / s, ties to even.  Infinities and
+// NaNs become e4m3's NaN and do not touch the block's other values.
+//
+// v / s must be the correctly rounded quotient: one step off moves values that lie next to a tie.  With r the correctly
+// rounded 1 / s and q0 = v r, q0 + r (v - q0 s) -- two fused operations -- is that quotient (Markstein, IBM J. Res. Dev. 34,
+// 1990), as long as the remainder does not underflow: it is a multiple of 2^-48 |v| at the least, and a value that is not
+// rounded to zero has |v| > 2^-11 s, so s >= 2^-80 is enough.  Blocks with a smaller scale divide.
+//
+// The maximum is taken on the 16-bit patterns, two at a time: without their sign, floats order as integers.  A block whose
+// maximum is not finite is gone through again, value by value.
 //
 // Bound by memory: two bytes read, one written per value, one pass (the block stays in registers between the maximum
 // and the quotients).
@@ -45,7 +52,19 @@ __device__ __forceinline__ uint4 load8(const uint16_t* p, int have) {
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __int_as_float(0x7f800000); }
 
-__device__ __forceinline__ float amax8(const float (&f)[8], float top) {
+// Largest magnitude of each half, as 16-bit patterns.
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t amax_pattern(uint4 v, uint32_t top) {
+    constexpr uint32_t kAbs = 0x7fff7fffu;
+    top = max_u16x2(top, max_u16x2(v.x & kAbs, v.y & kAbs));
+    return max_u16x2(top, max_u16x2(v.z & kAbs, v.w & kAbs));
+}
+
+__device__ __forceinline__ float amax_finite(const float (&f)[8], float top) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = finite(f[i]) ? fmaxf(top, fabsf(f[i])) : top;
     return top;
@@ -53,18 +72,45 @@ __device__ __forceinline__ float amax8(const float (&f)[8], float top) {
 
 __device__ __forceinline__ float scale_of(float amax) { return amax > 0.f ? fmaxf(amax / kE4m3Max, kScaleMin) : 1.f; }
 
-__device__ __forceinline__ uint2 quantize8(const float (&f)[8], float scale) {
+// What a block's values need to become e4m3: plain (all values finite, scale not tiny) takes the short way.
+struct BlockScale {
+    float scale, inverse;
+    bool plain;
+};
+__device__ __forceinline__ BlockScale block_scale(float amax, bool all_finite) {
+    BlockScale b;
+    b.scale = scale_of(amax);
+    b.inverse = 1.f / b.scale;
+    b.plain = all_finite && b.scale >= 8.2718061e-25f;      // 2^-80
+    return b;
+}
+
+__device__ __forceinline__ uint2 quantize8(const float (&f)[8], const BlockScale& b) {
+    float q[8];
+    if (b.plain) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float q0 = f[i] * b.inverse;
+            q[i] = fmaf(fmaf(-q0, b.scale, f[i]), b.inverse, q0);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = finite(f[i]) ? f[i] / b.scale : __int_as_float(0x7fffffff);
+    }
     uint32_t h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float nan = __int_as_float(0x7fffffff);
-        const float lo = finite(f[2 * i]) ? f[2 * i] / scale : nan, hi = finite(f[2 * i + 1]) ? f[2 * i + 1] / scale : nan;
         uint16_t t;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(t) : "f"(hi), "f"(lo));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(t) : "f"(q[2 * i + 1]), "f"(q[2 * i]));
         h[i] = t;
     }
     return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
 }
+
+__device__ __forceinline__ float pattern_value(uint32_t h, bool bf16) {
+    return bf16 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
+}
+__device__ __forceinline__ bool pattern_finite(uint32_t h, bool bf16) { return h < (bf16 ? 0x7f80u : 0x7c00u); }
 
 __device__ __forceinline__ void store8(unsigned char* p, int have, uint2 v) {
     if (have >= 8) { *reinterpret_cast<uint2*>(p) = v; return; }
@@ -93,15 +139,24 @@ k_quantize_rows(int bf16, uint64_t n_rows, const uint64_t* __restrict__ n_used, 
     for (int i = 0; i < kRowsPerWarp; ++i) v[i] = row0 + i < rows ? load8(in + (row0 + i) * ld_in + col, have) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i) {
+        uint32_t top = amax_pattern(v[i], 0u);
+#pragma unroll
+        for (int d = 8; d; d >>= 1) top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, d));
+        top = max(top & 0xffffu, top >> 16);
         float f[8];
         unpack8(v[i], bf16 != 0, f);
-        float top = amax8(f, 0.f);
+        const bool all_finite = pattern_finite(top, bf16 != 0);
+        float amax = pattern_value(top, bf16 != 0);
+        if (!__all_sync(0xffffffffu, all_finite)) {
+            float a = amax_finite(f, 0.f);
 #pragma unroll
-        for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        const float scale = scale_of(top);
+            for (int d = 8; d; d >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
+            amax = a;
+        }
+        const BlockScale b = block_scale(amax, all_finite);
         if (row0 + i < rows) {
-            if (have > 0) store8(out + (row0 + i) * ld_out + col, have, quantize8(f, scale));
-            if ((lane & 15) == 0 && block * 128 < n_cols) scales[(uint64_t)block * n_rows + row0 + i] = scale;
+            if (have > 0) store8(out + (row0 + i) * ld_out + col, have, quantize8(f, b));
+            if ((lane & 15) == 0 && block * 128 < n_cols) scales[(uint64_t)block * n_rows + row0 + i] = b.scale;
         }
     }
 }
@@ -118,30 +173,46 @@ k_quantize_weights(int bf16, uint32_t n_rows, uint32_t n_cols, const uint16_t* _
     uint4 v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = row0 + 16 * i < n_rows ? load8(in + (uint64_t)(row0 + 16 * i) * ld_in + col, have) : make_uint4(0u, 0u, 0u, 0u);
-    float top = 0.f;
+    __shared__ uint32_t sh[8];
+    __shared__ float sh_finite[8];
+    const int warp = threadIdx.x >> 5;
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float f[8];
-        unpack8(v[i], bf16 != 0, f);
-        top = amax8(f, top);
-    }
+    for (int i = 0; i < 8; ++i) top = amax_pattern(v[i], top);
 #pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    __shared__ float sh[8];
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = top;
+    for (int d = 16; d; d >>= 1) top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if ((threadIdx.x & 31) == 0) sh[warp] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, sh[i]);
-    const float scale = scale_of(top);
+    for (int i = 0; i < 8; ++i) top = max_u16x2(top, sh[i]);
+    top = max(top & 0xffffu, top >> 16);
+    const bool all_finite = pattern_finite(top, bf16 != 0);
+    float amax = pattern_value(top, bf16 != 0);
+    if (!all_finite) {                                  // the same for the whole CTA
+        amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float f[8];
+            unpack8(v[i], bf16 != 0, f);
+            amax = amax_finite(f, amax);
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+        if ((threadIdx.x & 31) == 0) sh_finite[warp] = amax;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, sh_finite[i]);
+    }
+    const BlockScale b = block_scale(amax, all_finite);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         if (row0 + 16 * i < n_rows && have > 0) {
             float f[8];
             unpack8(v[i], bf16 != 0, f);
-            store8(out + (uint64_t)(row0 + 16 * i) * ld_out + col, have, quantize8(f, scale));
+            store8(out + (uint64_t)(row0 + 16 * i) * ld_out + col, have, quantize8(f, b));
         }
     }
-    if (threadIdx.x == 0) scales[((uint64_t)mat * gridDim.y + by) * gridDim.x + bx] = scale;
+    if (threadIdx.x == 0) scales[((uint64_t)mat * gridDim.y + by) * gridDim.x + bx] = b.scale;
 }
 
 }  // namespace

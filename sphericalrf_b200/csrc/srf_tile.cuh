@@ -124,78 +124,77 @@ __host__ __device__ constexpr uint32_t idesc_shape(uint32_t n) { return (1u << 4
 // ---- ragged groups ----
 
 // Samples [begin, end) of group g.  Offsets that point behind the buffers or run backwards are cut to what is there
-// (every access stays in bounds) and reported through *bad.
-struct Span { uint64_t begin, end; };
-__device__ __forceinline__ Span group_span(const uint64_t* __restrict__ offsets, uint32_t g, uint64_t n_rows, bool* bad) {
+// (every access stays in bounds) and reported through *bad.  n_rows < 2^31.
+struct Span { uint32_t begin, end; };
+__device__ __forceinline__ Span group_span(const uint64_t* __restrict__ offsets, uint32_t g, uint32_t n_rows, bool* bad) {
     Span s = {0, n_rows};
     if (offsets) {
-        s.begin = __ldg((const unsigned long long*)offsets + g);
-        s.end = __ldg((const unsigned long long*)offsets + g + 1);
-        if (s.begin > s.end || s.end > n_rows) *bad = true;
-        s.end = s.end < n_rows ? s.end : n_rows;
-        s.begin = s.begin < s.end ? s.begin : s.end;
+        const uint64_t b = __ldg((const unsigned long long*)offsets + g), e = __ldg((const unsigned long long*)offsets + g + 1);
+        if (b > e || e > n_rows) *bad = true;
+        s.end = e < n_rows ? (uint32_t)e : n_rows;
+        s.begin = b < s.end ? (uint32_t)b : s.end;
     }
     return s;
 }
 
 // Walks the groups in windows of 32, one group per lane: unit u of the concatenation of all groups' units belongs to
 // the group whose running sum first exceeds u.  Units are asked for in ascending order, so a window is never revisited.
-// `units(span)` gives a group's number of units.
+// `units(span)` gives a group's number of units; all groups together have less than 2^32 (arrays end at 2^40 bytes).
 struct GroupWalk {
-    uint64_t base = 0;       // units in front of the window
-    uint64_t incl = 0;       // lane: units of the window up to and with this lane's group
-    uint64_t total = 0;      // units of the window
+    uint32_t base = 0;       // units in front of the window
+    uint32_t incl = 0;       // lane: units of the window up to and with this lane's group
+    uint32_t own = 0;        // lane: units of this lane's group
+    uint32_t total = 0;      // units of the window
     uint32_t g0 = 0;
     Span span = {0, 0};
     bool loaded = false;
 
     // Warp-collective.  False when there is no unit u.
     template <class Units>
-    __device__ __forceinline__ bool find(uint64_t u, const uint64_t* offsets, uint32_t n_groups, uint64_t n_rows, Units units,
-                                         uint32_t* group, Span* where, uint64_t* local, bool* bad) {
+    __device__ __forceinline__ bool find(uint32_t u, const uint64_t* offsets, uint32_t n_groups, uint32_t n_rows, Units units,
+                                         uint32_t* group, Span* where, uint32_t* local, bool* bad) {
         const uint32_t lane = threadIdx.x & 31;
         for (;;) {
             if (!loaded) {
                 if (g0 >= n_groups) return false;
                 span = {0, 0};
-                incl = 0;
+                own = 0;
                 if (g0 + lane < n_groups) {
                     span = group_span(offsets, g0 + lane, n_rows, bad);
-                    incl = units(span);
+                    own = units(span);
                 }
+                incl = own;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
-                    const uint64_t v = __shfl_up_sync(0xffffffffu, incl, d);
+                    const uint32_t v = __shfl_up_sync(0xffffffffu, incl, d);
                     if ((int)lane >= d) incl += v;
                 }
                 total = __shfl_sync(0xffffffffu, incl, 31);
                 loaded = true;
             }
-            if (u < base + total) break;
+            if (u - base < total) break;
             base += total;
             g0 += 32;
             loaded = false;
         }
-        const uint32_t hit = __ballot_sync(0xffffffffu, base + incl > u);
-        const int src = __ffs((int)hit) - 1;
-        const uint64_t before = __shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, units(span), src);
+        const int src = __ffs((int)__ballot_sync(0xffffffffu, incl > u - base)) - 1;
         where->begin = __shfl_sync(0xffffffffu, span.begin, src);
         where->end = __shfl_sync(0xffffffffu, span.end, src);
         *group = g0 + (uint32_t)src;
-        *local = u - base - before;
+        *local = u - base - __shfl_sync(0xffffffffu, incl - own, src);
         return true;
     }
 };
 
 // Output tile `local` of a group of mt x nt tiles -> (m, n).  Tiles run down bands of 16 row tiles, so that the tiles
 // in flight at one time share both operands in L2.
-__device__ __forceinline__ void tile_place(uint64_t local, uint64_t mt, uint32_t nt, uint64_t* m, uint32_t* n) {
-    const uint64_t band = local / (16ull * nt);
-    const uint64_t m0 = band * 16;
-    const uint32_t height = (uint32_t)(mt - m0 < 16 ? mt - m0 : 16);
-    const uint32_t r = (uint32_t)(local - band * 16ull * nt);
-    *m = m0 + r % height;
+__device__ __forceinline__ void tile_place(uint32_t local, uint32_t mt, uint32_t nt, uint32_t* m, uint32_t* n) {
+    const uint32_t band = local / (16u * nt);
+    const uint32_t m0 = band * 16;
+    const uint32_t height = mt - m0 < 16 ? mt - m0 : 16;
+    const uint32_t r = local - m0 * nt;
     *n = r / height;
+    *m = m0 + r - *n * height;
 }
 
 // ---- storing a finished piece of a tile ----
@@ -231,56 +230,93 @@ __device__ __forceinline__ void stage_unit(unsigned char* stage, int row, int un
     *reinterpret_cast<uint4*>(stage + row * 128 + ((unit ^ (row & 7)) << 4)) = v;
 }
 
-// Staged rows -> memory; the whole warp.
-__device__ __forceinline__ void store_rows(const RowStore& s, const unsigned char* stage) {
+// Shuts outputs whose gate is not > 0: `w` holds 16 bytes of output, `h` the gate's values for them.
+__device__ __forceinline__ uint4 gate_unit(uint4 w, uint4 h, bool f32, bool bf16) {
+    uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    const uint32_t g[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (f32) {
+            if (!positive16((g[e >> 1] >> ((e & 1) * 16)) & 0xffffu, bf16)) v[e] = 0u;
+        } else {
+            if (!positive16(g[e] & 0xffffu, bf16)) v[e] &= 0xffff0000u;
+            if (!positive16(g[e] >> 16, bf16)) v[e] &= 0x0000ffffu;
+        }
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// The gate's values of the units this lane will store, asked for before the tile's sums are ready.
+__device__ __forceinline__ void load_gate(const RowStore& s, uint4 (&hv)[8]) {
     const int lane = threadIdx.x & 31, unit = lane & 7;
+    const uint32_t from = (uint32_t)unit * 16u;
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {
+        const uint32_t row = (uint32_t)(it * 4 + (lane >> 3));
+        hv[it] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < s.rows && from < s.bytes) {
+            const unsigned char* gp = s.gate + row * s.gate_row_bytes + (s.f32 ? unit * 8 : unit * 16);
+            const uint32_t have = s.bytes - from;
+            if (have >= 16u) {
+                if (s.f32) {
+                    const uint2 t = __ldg(reinterpret_cast<const uint2*>(gp));
+                    hv[it] = make_uint4(t.x, t.y, 0u, 0u);
+                } else {
+                    hv[it] = __ldg(reinterpret_cast<const uint4*>(gp));
+                }
+            } else {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(gp);
+                const uint32_t n = s.f32 ? have / 4u : have / 2u;
+                uint32_t t[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if ((uint32_t)e < n) t[e >> 1] |= (uint32_t)__ldg(h + e) << ((e & 1) * 16);
+                hv[it] = make_uint4(t[0], t[1], t[2], t[3]);
+            }
+        }
+    }
+}
+
+// Staged rows -> memory; the whole warp.
+template <bool GATE>
+__device__ __forceinline__ void store_rows(const RowStore& s, const unsigned char* stage, const uint4 (&hv)[8]) {
+    const int lane = threadIdx.x & 31, unit = lane & 7;
+    const uint32_t from = (uint32_t)unit * 16u;
+    uint4 v[8];
     __syncwarp();
 #pragma unroll
     for (int it = 0; it < 8; ++it) {
         const uint32_t row = (uint32_t)(it * 4 + (lane >> 3));
-        if (row < s.rows && (uint32_t)unit * 16u < s.bytes) {
-            uint4 v = *reinterpret_cast<const uint4*>(stage + row * 128 + ((unit ^ (row & 7)) << 4));
-            unsigned char* p = s.out + row * s.row_bytes + unit * 16;
-            const uint32_t have = s.bytes - (uint32_t)unit * 16u;       // > 0
-            uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            if (s.gate) {
-                const unsigned char* gp = s.gate + row * s.gate_row_bytes;
+        v[it] = *reinterpret_cast<const uint4*>(stage + row * 128 + ((unit ^ (row & 7)) << 4));
+    }
+    __syncwarp();
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {
+        const uint32_t row = (uint32_t)(it * 4 + (lane >> 3));
+        if (row < s.rows && from < s.bytes) {
+            if (GATE) v[it] = gate_unit(v[it], hv[it], s.f32, s.bf16);
+            unsigned char* p = s.out + row * s.row_bytes + from;
+            const uint32_t have = s.bytes - from;
+            if (have >= 16u) {
+                *reinterpret_cast<uint4*>(p) = v[it];
+            } else {
+                const uint32_t w[4] = {v[it].x, v[it].y, v[it].z, v[it].w};
                 if (s.f32) {
-                    const uint16_t* h = reinterpret_cast<const uint16_t*>(gp + unit * 8);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if ((uint32_t)e * 4u < have && !positive16(h[e], s.bf16)) w[e] = 0u;
+                        if ((uint32_t)e * 4u < have) reinterpret_cast<uint32_t*>(p)[e] = w[e];
                 } else {
-                    const uint16_t* h = reinterpret_cast<const uint16_t*>(gp + unit * 16);
-                    uint4 hv = make_uint4(0u, 0u, 0u, 0u);
-                    if (have >= 16u) hv = __ldg(reinterpret_cast<const uint4*>(h));
-                    else {
-                        uint32_t t[4] = {0u, 0u, 0u, 0u};
-                        for (uint32_t e = 0; e * 2u < have; ++e) t[e >> 1] |= (uint32_t)h[e] << ((e & 1u) * 16);
-                        hv = make_uint4(t[0], t[1], t[2], t[3]);
-                    }
-                    const uint32_t hw[4] = {hv.x, hv.y, hv.z, hv.w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (!positive16(hw[e] & 0xffffu, s.bf16)) w[e] &= 0xffff0000u;
-                        if (!positive16(hw[e] >> 16, s.bf16)) w[e] &= 0x0000ffffu;
-                    }
+                    for (int e = 0; e < 8; ++e)
+                        if ((uint32_t)e * 2u < have) reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(w[e >> 1] >> ((e & 1) * 16));
                 }
-            }
-            if (have >= 16u) {
-                *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-            } else if (s.f32) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if ((uint32_t)e * 4u < have) reinterpret_cast<uint32_t*>(p)[e] = w[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if ((uint32_t)e * 2u < have) reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(w[e >> 1] >> ((e & 1) * 16));
             }
         }
     }
-    __syncwarp();
+}
+__device__ __forceinline__ void store_rows(const RowStore& s, const unsigned char* stage) {
+    const uint4 none[8] = {};
+    store_rows<false>(s, stage, none);
 }
 
 }  // namespace tile

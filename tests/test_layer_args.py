@@ -125,6 +125,7 @@ def test_gradient_refusals(drv):
     assert "d_gate" in ask(drv.input_grad, layer(), OFF, Y, W, G8 + 2, X)
     f32 = dict(out_type=abi.TYPE_F32)
     assert "2^26" in ask(drv.weight_grad, layer(n_rows=(1 << 26) + 1, **f32), OFF, Y, X, W, SP, 1 << 20)
+    assert "too large" in ask(drv.weight_grad, layer(n_rows=1 << 22, n_in=65536, n_out=65536, **f32), OFF, Y, X, W, SP, 1 << 20)
     assert "d_workspace is NULL" in ask(drv.weight_grad, layer(**f32), OFF, Y, X, W, None, 0)
     assert "overlaps d_workspace" in ask(drv.weight_grad, layer(**f32), OFF, Y, X, W, W, 1 << 20)
     assert "d_workspace overlaps d_x" in ask(drv.weight_grad, layer(**f32), OFF, Y, X, W, X, 1 << 20)
