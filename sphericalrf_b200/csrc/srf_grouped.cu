@@ -8,16 +8,18 @@
 //   weight grad  dW[g][n][k] = sum_r dy[r][n] x[r][k]         A, B = both sample arrays, read down their columns
 //
 // One persistent CTA per SM: a TMA warp fills a ring of 64-deep operand stages, one thread issues tcgen05.mma
-// (M = 128, N = BN, fp32 accumulator in TMEM, two accumulators), four warps take a finished accumulator to memory while
-// the next one fills.  Operands that are read down their columns stay as they lie in memory: the tensor core takes them
-// MN-major.  Tiles are dealt round-robin; every warp finds its tiles itself from the offsets (GroupWalk), so no launch,
-// workspace or host read prepares them.
+// (128 x BN outputs a CTA, fp32 accumulators in TMEM, two to four of them), two sets of four warps take finished
+// accumulators to memory, every other tile each, while the next ones fill.  Operands that are read down their columns
+// stay as they lie in memory: the tensor core takes them MN-major.  Tiles are dealt round-robin; every warp finds its
+// tiles itself from the offsets (GroupWalk), so no launch, workspace or host read prepares them.
+//
+// Large layers run on pairs of CTAs (CG = 2): one instruction computes 256 x 256 outputs on two SMs, each of which
+// loads its own 128 rows of A and half of B, so that an operand byte from L2 serves twice as many products.
 //
 // A tile's rows behind its group's end hold the next group's samples: harmless in the first two products (an output row
 // depends on its own sample alone and those rows are not stored).  In the weight gradient they would be summed, so the
 // rows of the last stage of a group are zeroed in shared memory, in both operands (a NaN of the next group must not
 // meet a zero).
-#include <cstdio>
 #include <cstring>
 #include "srf_layers.cuh"
 #include "srf_tile.cuh"
@@ -41,32 +43,31 @@ struct GroupedArgs {
     const uint64_t* offsets;
     unsigned char* out;
     const unsigned char* gate;
-    float* partial;               // weight gradient: two tiles of partial sums per CTA
+    float* partial;               // weight gradient: two tiles of partial sums per worker
     uint64_t out_row_bytes, out_group_bytes, gate_row_bytes;
     uint32_t n_rows, n_groups;
     uint32_t out_rows;            // weight gradient: n_out
     uint32_t out_cols;            // n_out, n_in, n_in
     uint32_t depth;               // summed length of the first two products
+    uint32_t n_workers;           // weight gradient: even shares of the work
     int bf16, f32, relu;
     unsigned int* error_flags;
 };
 
-template <int BN>
-__host__ __device__ constexpr int n_stages() { return BN == 256 ? 4 : BN == 128 ? 6 : 8; }
-template <int BN>
-__host__ __device__ constexpr int n_accs() { return BN == 256 ? 2 : 4; }
-template <int BN>
-__host__ __device__ constexpr int smem_bytes() {
-    const int b = 1024 + n_stages<BN>() * (kABytes + BN * kBK * 2) + kStoreBytes + 512;
+// CG CTAs share a tile of CG*128 x BN outputs; each holds 128 rows of A and BN/CG rows of B per stage.
+template <int BN, int CG> __host__ __device__ constexpr int n_stages() { return BN / CG == 256 ? 4 : BN / CG == 128 ? 6 : 8; }
+template <int BN> __host__ __device__ constexpr int n_accs() { return BN == 256 ? 2 : 4; }
+template <int BN, int CG> __host__ __device__ constexpr int smem_bytes() {
+    const int b = 1024 + n_stages<BN, CG>() * (kABytes + BN / CG * kBK * 2) + kStoreBytes + 512;
     return b < kSmemMin ? kSmemMin : b;
 }
 
 // Units of work of a group: whole output tiles for the first two products; 64-sample stages of output tiles for the
 // weight gradient, whose work is cut evenly across the CTAs (see below).
-template <int MODE>
+template <int MODE, int CG>
 __device__ __forceinline__ uint32_t group_units(const Span& s, uint32_t tiles_across) {
     const uint32_t rows = s.end - s.begin;
-    return (MODE == kWeightGrad ? (rows + kBK - 1) / kBK : (rows + kBM - 1) / kBM) * tiles_across;
+    return (MODE == kWeightGrad ? (rows + kBK - 1) / kBK : (rows + CG * kBM - 1) / (CG * kBM)) * tiles_across;
 }
 
 // One stretch of summed stages of one output tile.
@@ -79,39 +80,50 @@ struct Piece {
     uint32_t k_stages;     // stages
     bool whole;            // the piece is the tile's whole sum
     bool first;            // the piece holds the tile's first stage
+    uint32_t worker;
 };
 
-// The pieces of this CTA, one after the other; every warp walks them for itself.
+// The pieces of this CTA (or pair), one after the other; every warp walks them for itself.
 //
-// Weight gradient: the stages of all tiles are one line of `units` which the CTAs share out evenly, so ragged groups
-// balance by themselves and a narrow layer (one tile per group) still fills every SM.  A tile that a boundary cuts
-// is summed from the CTAs' partial sums, in the CTAs' order, by a second kernel: the same result on every run.
-__device__ __forceinline__ uint32_t first_unit(uint32_t units, uint32_t cta, uint32_t n_ctas) {
-    const uint32_t q = units / n_ctas, r = units - q * n_ctas;
-    return cta * q + (cta < r ? cta : r);
+// Weight gradient: the stages of all tiles are one line of `units` that n_workers share out evenly, so ragged groups
+// balance by themselves and a narrow layer (one tile per group) still fills every SM.  CTA c works for the workers c,
+// c + CTAs, ...: with more workers than CTAs, all CTAs are in the same part of the line at a time and find that part's
+// samples in L2.  A tile that a boundary cuts is summed from the workers' partial sums, in the workers' order, by a second
+// kernel: the same result on every run.
+__device__ __forceinline__ uint32_t first_unit(uint32_t units, uint32_t worker, uint32_t n_workers) {
+    const uint32_t q = units / n_workers, r = units - q * n_workers;
+    return worker * q + (worker < r ? worker : r);
 }
 
-template <int MODE>
+template <int MODE, int CG>
 struct Pieces {
     GroupWalk walk;
-    uint32_t at, stop, step;
-    // first two products: pieces start, start + step, ... of those dealt to this CTA
-    __device__ __forceinline__ void init(uint32_t units, uint32_t start, uint32_t every) {
+    uint32_t at, stop, step, units, worker;
+    // first two products: pieces start, start + every, ... of those dealt to this CTA
+    __device__ __forceinline__ void init(const GroupedArgs& p, uint32_t n_units, uint32_t start, uint32_t every) {
+        const uint32_t self = blockIdx.x / CG, all = gridDim.x / CG;
         if (MODE == kWeightGrad) {
-            at = first_unit(units, blockIdx.x, gridDim.x);
-            stop = first_unit(units, blockIdx.x + 1, gridDim.x);
-            step = 0;
+            units = n_units;
+            worker = self;
+            at = first_unit(units, worker, p.n_workers);
+            stop = first_unit(units, worker + 1, p.n_workers);
         } else {
-            at = blockIdx.x + start * gridDim.x;
-            stop = 0xffffffffu;
-            step = every * gridDim.x;
+            at = self + start * all;
+            step = every * all;
         }
     }
     __device__ __forceinline__ bool next(const GroupedArgs& p, uint32_t tiles_m, uint32_t tiles_n, Piece* o, bool* bad) {
-        if (at >= stop) return false;
+        if (MODE == kWeightGrad) {
+            while (at >= stop) {
+                worker += gridDim.x / CG;
+                if (worker >= p.n_workers) return false;
+                at = first_unit(units, worker, p.n_workers);
+                stop = first_unit(units, worker + 1, p.n_workers);
+            }
+        }
         const uint32_t across = MODE == kWeightGrad ? tiles_m * tiles_n : tiles_n;
         uint32_t local;
-        if (!walk.find(at, p.offsets, p.n_groups, p.n_rows, [&](const Span& s) { return group_units<MODE>(s, across); },
+        if (!walk.find(at, p.offsets, p.n_groups, p.n_rows, [&](const Span& s) { return group_units<MODE, CG>(s, across); },
                        &o->group, &o->span, &local, bad))
             return false;
         const uint32_t rows = o->span.end - o->span.begin;
@@ -120,15 +132,16 @@ struct Pieces {
             const uint32_t deep = (rows + kBK - 1) / kBK;
             const uint32_t t = local / deep;
             tile_place(t, tiles_m, tiles_n, &m, &o->n);
-            o->m = m * kBM;
+            o->m = m * (CG * kBM);
             o->k0 = local - t * deep;
             o->k_stages = deep - o->k0 < stop - at ? deep - o->k0 : stop - at;
             o->first = o->k0 == 0;
             o->whole = o->k_stages == deep;
+            o->worker = worker;
             at += o->k_stages;
         } else {
-            tile_place(local, (rows + kBM - 1) / kBM, tiles_n, &m, &o->n);
-            o->m = o->span.begin + m * kBM;
+            tile_place(local, (rows + CG * kBM - 1) / (CG * kBM), tiles_n, &m, &o->n);
+            o->m = o->span.begin + m * (CG * kBM);
             o->k0 = 0;
             o->k_stages = (p.depth + kBK - 1) / kBK;
             o->first = o->whole = true;
@@ -139,20 +152,29 @@ struct Pieces {
 };
 
 // Units of all groups (warp-collective).
-template <int MODE>
+template <int MODE, int CG>
 __device__ __forceinline__ uint32_t all_units(const GroupedArgs& p, uint32_t across, bool* bad) {
     uint32_t sum = 0;
-    for (uint32_t g = threadIdx.x & 31; g < p.n_groups; g += 32) sum += group_units<MODE>(group_span(p.offsets, g, p.n_rows, bad), across);
+    for (uint32_t g = threadIdx.x & 31; g < p.n_groups; g += 32) sum += group_units<MODE, CG>(group_span(p.offsets, g, p.n_rows, bad), across);
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     return sum;
 }
 
-template <int MODE, int BN>
+// Zeroes rows [r0, r1) of the blocks of 64 columns of an operand stage (128 bytes a row).
+__device__ __forceinline__ void zero_rows(unsigned char* stage, int blocks, int r0, int r1) {
+    const int units = (r1 - r0) * 8;
+    for (int i = threadIdx.x & 31; i < units * blocks; i += 32) {
+        const int blk = i / units, u = i - blk * units;
+        *reinterpret_cast<uint4*>(stage + blk * 8192 + r0 * 128 + u * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+
+template <int MODE, int BN, int CG>
 __global__ void __launch_bounds__(kThreads, 1)
 k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GroupedArgs p) {
-    constexpr int kStages = n_stages<BN>(), kAccs = n_accs<BN>();
-    constexpr int kBBytes = BN * kBK * 2;
+    constexpr int kStages = n_stages<BN, CG>(), kAccs = n_accs<BN>();
+    constexpr int kBRows = BN / CG, kBBytes = kBRows * kBK * 2;
     constexpr bool kAColumns = MODE == kWeightGrad, kBColumns = MODE != kLayer;     // read down the columns: MN-major
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -160,68 +182,91 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     unsigned char* sm_b = smem + kStages * kABytes;
     unsigned char* sm_store = sm_b + kStages * kBBytes;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm_store + kStoreBytes);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2 * kAccs);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2 * kAccs + 1);
     volatile uint32_t* failed = tmem_slot + 1;
     const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kStages;
     const uint32_t bar_acc_full = bar_empty + 8 * kStages, bar_acc_empty = bar_acc_full + 8 * kAccs;
+    const uint32_t bar_tail = bar_acc_empty + 8 * kAccs;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 2 ? cluster_rank() : 0;
     const uint32_t tiles_n = (p.out_cols + BN - 1) / BN;
-    const uint32_t tiles_m = MODE == kWeightGrad ? (p.out_rows + kBM - 1) / kBM : 0;
+    const uint32_t tiles_m = MODE == kWeightGrad ? (p.out_rows + CG * kBM - 1) / (CG * kBM) : 0;
 
+    // Barriers of a pair: `full` and `acc_empty` are those of rank 0, where the instructions are issued; `empty` and
+    // `acc_full` are signalled in both CTAs.
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
-        for (int i = 0; i < kAccs; ++i) { mbar_init(bar_acc_full + 8 * i, 1); mbar_init(bar_acc_empty + 8 * i, 4); }
+        for (int i = 0; i < kStages; ++i) { mbar_init(bar_full + 8 * i, CG); mbar_init(bar_empty + 8 * i, 1); }
+        for (int i = 0; i < kAccs; ++i) { mbar_init(bar_acc_full + 8 * i, 1); mbar_init(bar_acc_empty + 8 * i, 4 * CG); }
+        mbar_init(bar_tail, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *failed = 0;
         tma_prefetch_map(&map_a);
         tma_prefetch_map(&map_b);
     }
-    if (warp == 2) tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    if (warp == 2) tmem_alloc<CG>(smem_u32(tmem_slot), kTmemCols);
     tc_fence_before();
-    __syncthreads();
+    if (CG == 2) cluster_sync(); else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
     bool bad = false, ok = true;
-    Pieces<MODE> pieces;
+    Pieces<MODE, CG> pieces;
     const bool storing = MODE != kWeightGrad && warp >= 4;       // the two sets of epilogue warps take every other piece
-    pieces.init(MODE == kWeightGrad ? all_units<MODE>(p, tiles_m * tiles_n, &bad) : 0, storing ? (warp - 4) >> 2 : 0, storing ? 2 : 1);
+    pieces.init(p, MODE == kWeightGrad ? all_units<MODE, CG>(p, tiles_m * tiles_n, &bad) : 0, storing ? (warp - 4) >> 2 : 0, storing ? 2 : 1);
     Piece t;
 
     if (warp == 0) {
         // ---- operand loads ----
+        const uint32_t lead_full = CG == 2 ? leader_addr(bar_full) : bar_full;
         uint32_t s = 0, round = 0;                     // ring position
-        uint32_t in_flight = 0;
+        uint32_t in_flight = 0, tails = 0;
         while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
+            const int am = (int)(t.m + rank * kBM), bn = (int)(t.n * BN + rank * kBRows);
             for (uint32_t k = 0; k < t.k_stages; ++k) {
                 if (round > 0 && !mbar_wait(bar_empty + 8 * s, (round - 1) & 1, failed)) { ok = false; break; }
+                const uint32_t rows = t.span.end - t.span.begin - (t.k0 + k) * kBK;      // weight gradient: samples from here on
+                const bool tail = MODE == kWeightGrad && rows < (uint32_t)kBK;
+                const uint32_t a = smem_u32(sm_a) + s * kABytes, b = smem_u32(sm_b) + s * kBBytes;
                 if (elect_one()) {
-                    const uint32_t bar = bar_full + 8 * s, a = smem_u32(sm_a) + s * kABytes, b = smem_u32(sm_b) + s * kBBytes;
-                    mbar_expect(bar, kABytes + kBBytes);
+                    const uint32_t bar = tail ? bar_tail : lead_full + 8 * s;
+                    if (tail) mbar_expect(bar_tail, kABytes + kBBytes);
+                    else pair_expect<CG>(bar, kABytes + kBBytes);
                     const int kk = (int)((t.k0 + k) * kBK);
                     if (kAColumns) {
 #pragma unroll
-                        for (int i = 0; i < kBM / 64; ++i) tma_2d(a + i * 8192, &map_a, bar, (int)t.m + 64 * i, (int)t.span.begin + kk);
+                        for (int i = 0; i < kBM / 64; ++i) tma_2d<CG>(a + i * 8192, &map_a, bar, am + 64 * i, (int)t.span.begin + kk);
                     } else {
-                        tma_2d(a, &map_a, bar, kk, (int)t.m);
+                        tma_2d<CG>(a, &map_a, bar, kk, am);
                     }
                     if (MODE == kLayer) {
-                        tma_3d(b, &map_b, bar, kk, (int)(t.n * BN), (int)t.group);
+                        tma_3d<CG>(b, &map_b, bar, kk, bn, (int)t.group);
                     } else if (MODE == kInputGrad) {
 #pragma unroll
-                        for (int i = 0; i < BN / 64; ++i) tma_3d(b + i * 8192, &map_b, bar, (int)(t.n * BN) + 64 * i, kk, (int)t.group);
+                        for (int i = 0; i < kBRows / 64; ++i) tma_3d<CG>(b + i * 8192, &map_b, bar, bn + 64 * i, kk, (int)t.group);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < BN / 64; ++i) tma_2d(b + i * 8192, &map_b, bar, (int)(t.n * BN) + 64 * i, (int)t.span.begin + kk);
+                        for (int i = 0; i < kBRows / 64; ++i) tma_2d<CG>(b + i * 8192, &map_b, bar, bn + 64 * i, (int)t.span.begin + kk);
                     }
                 }
                 __syncwarp();
+                if (tail) {
+                    // The group's last stage: when it has landed, zero the next group's samples up to the next 16 (an
+                    // instruction's depth), then report the stage.
+                    if (!mbar_wait(bar_tail, tails++ & 1, failed)) { ok = false; break; }
+                    const int r0 = (int)rows, r1 = (r0 + 15) & ~15;
+                    zero_rows(sm_a + s * kABytes, kBM / 64, r0, r1);
+                    zero_rows(sm_b + s * kBBytes, kBRows / 64, r0, r1);
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) pair_arrive<CG>(lead_full + 8 * s);
+                    __syncwarp();
+                }
                 if (++s == kStages) { s = 0; ++round; }
                 in_flight = in_flight < kStages ? in_flight + 1 : in_flight;
             }
         }
-        // Copies may still be on their way when another warp gave up: they must land before the CTA leaves.
-        if (!ok || *failed) {
+        // Copies may still be on their way when another warp gave up: they must land before the CTA (or pair) leaves.
+        if ((!ok || *failed) && rank == 0) {
             for (uint32_t i = 0; i < in_flight; ++i) {
                 const uint32_t q = s >= i + 1 ? s - i - 1 : s + kStages - i - 1;
                 const uint32_t r = s >= i + 1 ? round : round - 1;
@@ -229,9 +274,9 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 mbar_wait(bar_full + 8 * q, r & 1, &none);
             }
         }
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0) {
         // ---- matrix instructions ----
-        const uint32_t idesc = idesc_shape(BN) | (p.bf16 ? (1u << 7) | (1u << 10) : 0u) | (kAColumns ? 1u << 15 : 0u) | (kBColumns ? 1u << 16 : 0u);
+        const uint32_t idesc = idesc_shape(CG * kBM, BN) | (p.bf16 ? (1u << 7) | (1u << 10) : 0u) | (kAColumns ? 1u << 15 : 0u) | (kBColumns ? 1u << 16 : 0u);
         uint32_t s = 0, round = 0, acc = 0, acc_round = 0;
         while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
             if (acc_round > 0 && !mbar_wait(bar_acc_empty + 8 * acc, (acc_round - 1) & 1, failed)) { ok = false; break; }
@@ -242,19 +287,10 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 tc_fence_after();
                 int k_steps = kBK / 16;
                 if (MODE == kWeightGrad) {
-                    const uint32_t left = t.span.end - t.span.begin - (t.k0 + k) * kBK;     // samples of this stage
-                    if (left < (uint32_t)kBK) {
-                        // the group's last stage: instructions cover whole 16s, so zero up to the next 16
-                        const int r0 = (int)left, r1 = (r0 + 15) & ~15;
-                        k_steps = r1 / 16;
-                        const int units = (r1 - r0) * 8;
-                        for (int i = lane; i < units * (kBM / 64 + BN / 64); i += 32) {
-                            const int blk = i / units, u = i - blk * units;
-                            unsigned char* base = blk < kBM / 64 ? sm_a + s * kABytes + blk * 8192 : sm_b + s * kBBytes + (blk - kBM / 64) * 8192;
-                            *reinterpret_cast<uint4*>(base + r0 * 128 + u * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        }
-                        fence_async_smem();
-                        __syncwarp();
+                    const uint32_t rows = t.span.end - t.span.begin - (t.k0 + k) * kBK;
+                    if (rows < (uint32_t)kBK) {
+                        k_steps = (int)(rows + 15) / 16;
+                        pair_acquire<CG>();                // the other CTA zeroed rows of its operands
                     }
                 }
                 if (elect_one()) {
@@ -262,10 +298,10 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     for (int q = 0; q < k_steps; ++q) {
                         const uint64_t da = kAColumns ? operand_desc(a + q * 2048, 8192, 1024) : operand_desc(a + q * 32, 16, 1024);
                         const uint64_t db = kBColumns ? operand_desc(b + q * 2048, 8192, 1024) : operand_desc(b + q * 32, 16, 1024);
-                        mma_f16(d, da, db, idesc, (k | (uint32_t)q) != 0);
+                        mma_f16<CG>(d, da, db, idesc, (k | (uint32_t)q) != 0);
                     }
-                    mma_commit(bar_empty + 8 * s);
-                    if (k + 1 == t.k_stages) mma_commit(bar_acc_full + 8 * acc);
+                    mma_commit<CG>(bar_empty + 8 * s);
+                    if (k + 1 == t.k_stages) mma_commit<CG>(bar_acc_full + 8 * acc);
                 }
                 __syncwarp();
                 if (++s == kStages) { s = 0; ++round; }
@@ -277,6 +313,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         // ---- finished accumulators to memory ----
         const int quarter = warp & 3, set = (warp - 4) >> 2;
         unsigned char* stage = sm_store + (warp - 4) * 4096;
+        const uint32_t lead_acc_empty = CG == 2 ? leader_addr(bar_acc_empty) : bar_acc_empty;
         uint32_t acc = set, acc_round = 0;
         if (MODE == kWeightGrad && set) pieces.next(p, tiles_m, tiles_n, &t, &bad);
         while (pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
@@ -287,15 +324,15 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             const bool partial = MODE == kWeightGrad && !t.whole;
             const bool gated = MODE == kInputGrad && p.gate;
             rs.f32 = partial || p.f32;
-            const uint32_t row0 = t.m + quarter * 32;
+            const uint32_t row0 = t.m + rank * kBM + quarter * 32;
             const uint32_t end = MODE == kWeightGrad ? p.out_rows : t.span.end;
             rs.rows = row0 >= end ? 0u : end - row0 < 32 ? end - row0 : 32u;
             const uint32_t col0 = t.n * BN;
             const uint32_t cols = p.out_cols - col0 < (uint32_t)BN ? p.out_cols - col0 : (uint32_t)BN;
             unsigned char* out;
             if (partial) {
-                // slot 0: the tile began in an earlier CTA; slot 1: it goes on in the next one
-                out = reinterpret_cast<unsigned char*>(p.partial + ((size_t)blockIdx.x * 2 + (t.first ? 1 : 0)) * kBM * BN) + (size_t)quarter * 32 * BN * 4;
+                // slot 0: the tile began with an earlier worker; slot 1: it goes on with the next one
+                out = reinterpret_cast<unsigned char*>(p.partial + (((size_t)t.worker * 2 + (t.first ? 1 : 0)) * CG + rank) * kBM * BN) + (size_t)quarter * 32 * BN * 4;
                 rs.row_bytes = BN * 4;
             } else {
                 out = p.out + (MODE == kWeightGrad ? t.group * p.out_group_bytes : 0ull) + row0 * p.out_row_bytes;
@@ -317,7 +354,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 uint32_t r[32];
                 if (rs.f32) {
                     tmem_ld32(d + c, r);
-                    tmem_ld_wait();
+                    tmem_ld_wait(r);
                     if (p.relu)
 #pragma unroll
                         for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(relu(__uint_as_float(r[i])));
@@ -328,7 +365,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     for (int h = 0; h < 2; ++h) {
                         if (c + 32u * h < cols) {
                             tmem_ld32(d + c + 32 * h, r);
-                            tmem_ld_wait();
+                            tmem_ld_wait(r);
                             if (p.relu)
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(relu(__uint_as_float(r[i])));
@@ -343,7 +380,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 if (c + per >= cols) {             // the accumulator is read: a later tile may have it
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(bar_acc_empty + 8 * acc);
+                    if (lane == 0) pair_arrive_read<CG>(lead_acc_empty + 8 * acc);
                 }
                 if (gated) {
                     store_rows<true>(rs, stage, hv);
@@ -363,25 +400,27 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     }
     if ((bad || (!ok && lane == 0)) && p.error_flags) atomicOr(p.error_flags, (ok ? 0u : 2u) | (bad ? 16u : 0u));
     tc_fence_before();
-    __syncthreads();
-    if (warp == 2) tmem_free(tmem, kTmemCols);
+    if (CG == 2) cluster_sync(); else __syncthreads();      // a pair's barriers and accumulators serve both CTAs to the end
+    if (warp == 2) tmem_free<CG>(tmem, kTmemCols);
 }
 
-// Second kernel of the weight gradient.  Blocks (c, slice) with c < n_ctas - 1: the boundary behind CTA c.  If it cuts an
-// output tile and is the first to cut it, sums the tile's partial sums in the CTAs' order (the slice: a few of its rows).
-// The other blocks (n_ctas - 1 + g, slice) write the zeros of a group without samples.
-constexpr int kJoinSlices = 16, kJoinThreads = 256;
+// Second kernel of the weight gradient.  Blocks (v, slice) with v < n_workers - 1: the boundary behind worker v.  If it
+// cuts an output tile and is the first to cut it, sums the tile's partial sums in the workers' order (the slice: a few of
+// its rows).  The other blocks (n_workers - 1 + g, slice) write the zeros of a group without samples.
+constexpr int kJoinThreads = 256;
+template <int BN, int CG> __host__ __device__ constexpr int join_slices() { return CG * BN / 16; }      // 2048 sums a block
 
-template <int BN>
-__global__ void __launch_bounds__(kJoinThreads) k_weight_grad_join(const GroupedArgs p, uint32_t n_ctas) {
-    const uint32_t tiles_n = (p.out_cols + BN - 1) / BN, tiles_m = (p.out_rows + kBM - 1) / kBM;
-    const uint32_t across = tiles_m * tiles_n, slice = blockIdx.y;
+template <int BN, int CG>
+__global__ void __launch_bounds__(kJoinThreads) k_weight_grad_join(const GroupedArgs p) {
+    constexpr uint32_t kSlices = join_slices<BN, CG>(), kRows = CG * kBM / kSlices, kQuads = kRows * BN / 4;
+    const uint32_t tiles_n = (p.out_cols + BN - 1) / BN, tiles_m = (p.out_rows + CG * kBM - 1) / (CG * kBM);
+    const uint32_t across = tiles_m * tiles_n, slice = blockIdx.y, n = p.n_workers;
     bool bad = false;
-    if (blockIdx.x >= n_ctas - 1) {
-        const uint32_t g = blockIdx.x - (n_ctas - 1);
+    if (blockIdx.x >= n - 1) {
+        const uint32_t g = blockIdx.x - (n - 1);
         const Span s = group_span(p.offsets, g, p.n_rows, &bad);
         if (s.end > s.begin) return;
-        for (uint32_t row = slice; row < p.out_rows; row += kJoinSlices) {
+        for (uint32_t row = slice; row < p.out_rows; row += kSlices) {
             unsigned char* o = p.out + g * p.out_group_bytes + row * p.out_row_bytes;
             for (uint32_t col = threadIdx.x; col < p.out_cols; col += kJoinThreads) {
                 if (p.f32) reinterpret_cast<float*>(o)[col] = 0.f;
@@ -390,82 +429,105 @@ __global__ void __launch_bounds__(kJoinThreads) k_weight_grad_join(const Grouped
         }
         return;
     }
-    __shared__ uint32_t sh[5];         // first and last CTA of the tile, its group, m, n
+    __shared__ uint32_t sh[5];         // first and last worker of the tile, its group, m, n
     if (threadIdx.x < 32) {
-        const uint32_t units = all_units<kWeightGrad>(p, across, &bad);
-        const uint32_t u = first_unit(units, blockIdx.x + 1, n_ctas);       // first unit behind the boundary
+        const uint32_t units = all_units<kWeightGrad, CG>(p, across, &bad);
+        const uint32_t u = first_unit(units, blockIdx.x + 1, n);       // first unit behind the boundary
         GroupWalk walk;
-        uint32_t group = 0, local = 0, c0 = 1, c1 = 0, m = 0, n = 0;
+        uint32_t group = 0, local = 0, v0 = 1, v1 = 0, tm = 0, tn = 0;
         Span s = {0, 0};
         if (u > 0 && u < units &&
-            walk.find(u, p.offsets, p.n_groups, p.n_rows, [&](const Span& q) { return group_units<kWeightGrad>(q, across); }, &group, &s, &local, &bad)) {
+            walk.find(u, p.offsets, p.n_groups, p.n_rows, [&](const Span& q) { return group_units<kWeightGrad, CG>(q, across); }, &group, &s, &local, &bad)) {
             const uint32_t deep = (s.end - s.begin + kBK - 1) / kBK, t = local / deep, k = local - t * deep;
-            const uint32_t u0 = u - k, before = first_unit(units, blockIdx.x, n_ctas);
+            const uint32_t u0 = u - k, before = first_unit(units, blockIdx.x, n);
             // the boundary cuts the tile, and the one in front of it does not
             if (k > 0 && before <= u0 && before < u) {
-                c0 = blockIdx.x;
-                c1 = c0 + 1;
-                while (c1 + 1 < n_ctas && first_unit(units, c1 + 1, n_ctas) < u0 + deep) ++c1;
-                tile_place(t, tiles_m, tiles_n, &m, &n);
+                v0 = blockIdx.x;
+                v1 = v0 + 1;
+                while (v1 + 1 < n && first_unit(units, v1 + 1, n) < u0 + deep) ++v1;
+                tile_place(t, tiles_m, tiles_n, &tm, &tn);
             }
         }
-        if (threadIdx.x == 0) { sh[0] = c0; sh[1] = c1; sh[2] = group; sh[3] = m; sh[4] = n; }
+        if (threadIdx.x == 0) { sh[0] = v0; sh[1] = v1; sh[2] = group; sh[3] = tm; sh[4] = tn; }
     }
     __syncthreads();
-    const uint32_t c0 = sh[0], c1 = sh[1];
-    if (c0 > c1) return;
-    constexpr uint32_t kRows = kBM / kJoinSlices, kQuads = kRows * BN / 4;
+    const uint32_t v0 = sh[0], v1 = sh[1];
+    if (v0 > v1) return;
     for (uint32_t i = threadIdx.x; i < kQuads; i += kJoinThreads) {
         const uint32_t row = slice * kRows + i / (BN / 4), col = i % (BN / 4) * 4;
-        const uint32_t orow = sh[3] * kBM + row, ocol = sh[4] * BN + col;
+        const uint32_t orow = sh[3] * (CG * kBM) + row, ocol = sh[4] * BN + col;
         if (orow >= p.out_rows || ocol >= p.out_cols) continue;
         const float4* q = reinterpret_cast<const float4*>(p.partial + (size_t)row * BN + col);
-        constexpr size_t kSlot = (size_t)kBM * BN / 4;
-        float4 sum = q[(2 * (size_t)c0 + 1) * kSlot];
+        constexpr size_t kSlot = (size_t)CG * kBM * BN / 4;
+        float4 sum = q[(2 * (size_t)v0 + 1) * kSlot];
 #pragma unroll 8
-        for (uint32_t c = c0 + 1; c <= c1; ++c) {
-            const float4 v = q[2 * (size_t)c * kSlot];
-            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        for (uint32_t v = v0 + 1; v <= v1; ++v) {
+            const float4 e = q[2 * (size_t)v * kSlot];
+            sum.x += e.x; sum.y += e.y; sum.z += e.z; sum.w += e.w;
         }
         unsigned char* o = p.out + sh[2] * p.out_group_bytes + orow * p.out_row_bytes;
         const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+        if (p.f32 && ocol + 4 <= p.out_cols) {
+            reinterpret_cast<float4*>(o)[ocol / 4] = sum;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (ocol + e >= p.out_cols) continue;
-            if (p.f32) reinterpret_cast<float*>(o)[ocol + e] = f[e];
-            else reinterpret_cast<uint16_t*>(o)[ocol + e] = (uint16_t)pack16(f[e], 0.f, p.bf16 != 0);
+            for (int e = 0; e < 4; ++e) {
+                if (ocol + e >= p.out_cols) continue;
+                if (p.f32) reinterpret_cast<float*>(o)[ocol + e] = f[e];
+                else reinterpret_cast<uint16_t*>(o)[ocol + e] = (uint16_t)pack16(f[e], 0.f, p.bf16 != 0);
+            }
         }
     }
 }
 
-// Width of the output tile: the widest that leaves every SM a few tiles (a wide tile reads its operands from L2 less
-// often, a narrow one spreads few tiles over more SMs).
-int pick_bn(uint64_t row_tiles, uint32_t cols, int sms, int smallest) {
-    int bn = 256;
-    while (bn > smallest && (((uint64_t)(bn / 2) >= cols) || row_tiles * ((cols + bn - 1) / bn) < 2ull * sms)) bn /= 2;
-    return bn;
+// Shape and shares of the weight gradient.
+struct WeightGradPlan { int bn, cg; uint64_t across; uint32_t grid, workers; };
+WeightGradPlan plan_weight_grad(const srf_grouped_t& p, int sms) {
+    WeightGradPlan w;
+    w.cg = p.n_out > 128 && p.n_in > 128 ? 2 : 1;
+    w.bn = p.n_in <= 64 ? 64 : p.n_in <= 128 ? 128 : 256;
+    w.across = (uint64_t)((p.n_out + w.cg * kBM - 1) / (w.cg * kBM)) * ((p.n_in + w.bn - 1) / w.bn);
+    const uint64_t units = max_row_tiles(p, kBK) * w.across, teams = sms / w.cg;
+    const uint64_t busy = units < teams ? units : teams;
+    // All teams together walk the samples once per tile of a group that a team works on; samples beyond what L2 holds are
+    // taken part by part.
+    const uint64_t bytes = p.n_rows * (p.n_in + p.n_out) * 2;
+    uint64_t parts = w.across < 8 ? 1 : bytes / (64ull << 20) + 1;
+    if (parts > 4) parts = 4;
+    w.grid = (uint32_t)busy * w.cg;
+    w.workers = (uint32_t)(busy * parts);
+    if (!w.workers) w.workers = 1;
+    return w;
 }
 
-template <int MODE, int BN>
-const char* launch(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& args, uint64_t max_units, cudaStream_t stream) {
-    static_assert(smem_bytes<BN>() <= 227 * 1024, "shared memory of one SM");
-    const int sms = sm_count();
-    if (cudaFuncSetAttribute((const void*)k_grouped<MODE, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<BN>()) != cudaSuccess)
-        return "cudaFuncSetAttribute failed";
-    const int grid = (int)(max_units < (uint64_t)sms ? max_units : (uint64_t)sms);
-    k_grouped<MODE, BN><<<grid, kThreads, smem_bytes<BN>(), stream>>>(a, b, args);
-    return nullptr;
+template <int MODE, int BN, int CG>
+const char* launch(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& args, uint32_t grid, cudaStream_t stream) {
+    static_assert(smem_bytes<BN, CG>() <= 227 * 1024, "shared memory of one SM");
+    return launch_tiles(k_grouped<MODE, BN, CG>, smem_bytes<BN, CG>(), kThreads, CG, grid, stream, a, b, args);
 }
-
-// Row tiles that n_rows samples in n_groups groups can have at most.
-uint64_t max_row_tiles(const srf_grouped_t& p) {
-    const uint64_t busy = p.n_groups < p.n_rows ? p.n_groups : p.n_rows;
-    return p.n_rows / kBM + busy;
-}
-
-int weight_grad_bn(const srf_grouped_t& p) { return p.n_in <= 64 ? 64 : p.n_in <= 128 ? 128 : 256; }
 
 }  // namespace
+
+uint64_t max_row_tiles(const srf_grouped_t& p, uint64_t height) {
+    const uint64_t busy = p.n_groups < p.n_rows ? p.n_groups : p.n_rows;
+    return p.n_rows / height + busy;
+}
+
+TileShape pick_tile(const srf_grouped_t& p, uint32_t cols, int sms, int smallest) {
+    // Pairs: groups of a few 256-row tiles at least, and enough tiles for every pair.
+    if (cols > 128 && p.n_rows / p.n_groups >= 512 && p.n_rows / 256 * ((cols + 255) / 256) >= (uint64_t)sms) return {256, 2};
+    // Otherwise the widest tile that leaves every SM a few (a wide tile reads its operands from L2 less often, a
+    // narrow one spreads few tiles over more SMs).
+    const uint64_t row_tiles = max_row_tiles(p, 128);
+    int bn = 256;
+    while (bn > smallest && ((uint32_t)bn / 2 >= cols || row_tiles * ((cols + bn - 1) / bn) < 2ull * sms)) bn /= 2;
+    return {bn, 1};
+}
+
+uint32_t tile_grid(const srf_grouped_t& p, uint32_t cols, TileShape t, int sms) {
+    const uint64_t tiles = max_row_tiles(p, t.cg * 128) * ((cols + t.bn - 1) / t.bn), teams = sms / t.cg;
+    return (uint32_t)(tiles < teams ? tiles : teams) * t.cg;
+}
 
 int sm_count() {
     int dev = 0, sms = 148;
@@ -500,32 +562,33 @@ bool make_operand_map(void* map, const void* base, int type, uint64_t cols, uint
 
 const char* launch_grouped_matmul(const srf_grouped_t& p, const uint64_t* offsets, const void* x, const void* w, void* y,
                                   unsigned int* error_flags, cudaStream_t stream) {
-    const uint64_t row_tiles = max_row_tiles(p);
-    if (!row_tiles) return nullptr;
-    const int bn = pick_bn(row_tiles, p.n_out, sm_count(), 32);
+    if (!p.n_rows) return nullptr;
+    const int sms = sm_count();
+    const TileShape t = pick_tile(p, p.n_out, sms, 32);
     CUtensorMap a, b;
     if (!make_operand_map(&a, x, p.type, p.n_in, p.n_rows, p.ld_x, 0, 0, kBM) ||
-        !make_operand_map(&b, w, p.type, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, bn))
+        !make_operand_map(&b, w, p.type, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, t.bn / t.cg))
         return "the driver refused an operand's tensor map";
     GroupedArgs k;
     memset(&k, 0, sizeof(k));
     k.offsets = offsets; k.out = (unsigned char*)y; k.n_rows = (uint32_t)p.n_rows; k.n_groups = p.n_groups;
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16; k.relu = p.activation == SRF_ACT_RELU;
     k.out_row_bytes = p.ld_y * (k.f32 ? 4 : 2); k.out_cols = p.n_out; k.depth = p.n_in; k.error_flags = error_flags;
-    const uint64_t units = row_tiles * ((p.n_out + bn - 1) / bn);
-    switch (bn) {
-    case 256: return launch<kLayer, 256>(a, b, k, units, stream);
-    case 128: return launch<kLayer, 128>(a, b, k, units, stream);
-    case 64: return launch<kLayer, 64>(a, b, k, units, stream);
-    default: return launch<kLayer, 32>(a, b, k, units, stream);
+    const uint32_t grid = tile_grid(p, p.n_out, t, sms);
+    if (t.cg == 2) return launch<kLayer, 256, 2>(a, b, k, grid, stream);
+    switch (t.bn) {
+    case 256: return launch<kLayer, 256, 1>(a, b, k, grid, stream);
+    case 128: return launch<kLayer, 128, 1>(a, b, k, grid, stream);
+    case 64: return launch<kLayer, 64, 1>(a, b, k, grid, stream);
+    default: return launch<kLayer, 32, 1>(a, b, k, grid, stream);
     }
 }
 
 const char* launch_grouped_input_grad(const srf_grouped_t& p, const uint64_t* offsets, const void* dy, const void* w,
                                       const void* gate, void* dx, unsigned int* error_flags, cudaStream_t stream) {
-    const uint64_t row_tiles = max_row_tiles(p);
-    if (!row_tiles) return nullptr;
-    const int bn = pick_bn(row_tiles, p.n_in, sm_count(), 64);
+    if (!p.n_rows) return nullptr;
+    const int sms = sm_count();
+    const TileShape t = pick_tile(p, p.n_in, sms, 64);
     CUtensorMap a, b;
     if (!make_operand_map(&a, dy, p.type, p.n_out, p.n_rows, p.ld_y, 0, 0, kBM) ||
         !make_operand_map(&b, w, p.type, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, kBK))
@@ -536,48 +599,55 @@ const char* launch_grouped_input_grad(const srf_grouped_t& p, const uint64_t* of
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16;
     k.out_row_bytes = p.ld_x * (k.f32 ? 4 : 2); k.gate_row_bytes = p.ld_x * 2; k.out_cols = p.n_in; k.depth = p.n_out;
     k.error_flags = error_flags;
-    const uint64_t units = row_tiles * ((p.n_in + bn - 1) / bn);
-    switch (bn) {
-    case 256: return launch<kInputGrad, 256>(a, b, k, units, stream);
-    case 128: return launch<kInputGrad, 128>(a, b, k, units, stream);
-    default: return launch<kInputGrad, 64>(a, b, k, units, stream);
+    const uint32_t grid = tile_grid(p, p.n_in, t, sms);
+    if (t.cg == 2) return launch<kInputGrad, 256, 2>(a, b, k, grid, stream);
+    switch (t.bn) {
+    case 256: return launch<kInputGrad, 256, 1>(a, b, k, grid, stream);
+    case 128: return launch<kInputGrad, 128, 1>(a, b, k, grid, stream);
+    default: return launch<kInputGrad, 64, 1>(a, b, k, grid, stream);
     }
 }
 
 size_t grouped_weight_grad_workspace(const srf_grouped_t& p, int n_sms) {
-    return (size_t)n_sms * 2 * kBM * weight_grad_bn(p) * sizeof(float);
+    const WeightGradPlan w = plan_weight_grad(p, n_sms);
+    return (size_t)w.workers * 2 * w.cg * kBM * w.bn * sizeof(float);
 }
+
+namespace {
+
+template <int BN, int CG>
+const char* weight_grad(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& k, uint32_t grid, cudaStream_t stream) {
+    if (grid) {
+        const char* why = launch<kWeightGrad, BN, CG>(a, b, k, grid, stream);
+        if (why) return why;
+    }
+    k_weight_grad_join<BN, CG><<<dim3(k.n_workers - 1 + k.n_groups, join_slices<BN, CG>()), kJoinThreads, 0, stream>>>(k);
+    return nullptr;
+}
+
+}  // namespace
 
 const char* launch_grouped_weight_grad(const srf_grouped_t& p, const uint64_t* offsets, const void* dy, const void* x, void* dw,
                                        void* workspace, unsigned int* error_flags, cudaStream_t stream) {
-    const int bn = weight_grad_bn(p);
+    const WeightGradPlan w = plan_weight_grad(p, sm_count());
     GroupedArgs k;
     memset(&k, 0, sizeof(k));
     k.offsets = offsets; k.out = (unsigned char*)dw; k.partial = (float*)workspace; k.n_rows = (uint32_t)p.n_rows; k.n_groups = p.n_groups;
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16;
     k.out_row_bytes = p.ld_w * (k.f32 ? 4 : 2); k.out_group_bytes = p.group_stride * (k.f32 ? 4 : 2);
-    k.out_rows = p.n_out; k.out_cols = p.n_in; k.error_flags = error_flags;
-    const uint64_t across = (uint64_t)((p.n_out + kBM - 1) / kBM) * ((p.n_in + bn - 1) / bn);
-    const uint64_t busy = p.n_groups < p.n_rows ? p.n_groups : p.n_rows;
-    const uint64_t units = (p.n_rows / kBK + busy) * across;
-    const int sms = sm_count();
-    const uint32_t grid = (uint32_t)(units < (uint64_t)sms ? units : (uint64_t)sms);
-    if (units) {
-        CUtensorMap a, b;
-        if (!make_operand_map(&a, dy, p.type, p.n_out, p.n_rows, p.ld_y, 0, 0, kBK) ||
-            !make_operand_map(&b, x, p.type, p.n_in, p.n_rows, p.ld_x, 0, 0, kBK))
-            return "the driver refused an operand's tensor map";
-        const char* why = bn == 256 ? launch<kWeightGrad, 256>(a, b, k, units, stream)
-                        : bn == 128 ? launch<kWeightGrad, 128>(a, b, k, units, stream)
-                                    : launch<kWeightGrad, 64>(a, b, k, units, stream);
-        if (why) return why;
+    k.out_rows = p.n_out; k.out_cols = p.n_in; k.n_workers = w.workers; k.error_flags = error_flags;
+    CUtensorMap a, b;
+    memset(&a, 0, sizeof(a));
+    memset(&b, 0, sizeof(b));
+    if (w.grid && (!make_operand_map(&a, dy, p.type, p.n_out, p.n_rows, p.ld_y, 0, 0, kBK) ||
+                   !make_operand_map(&b, x, p.type, p.n_in, p.n_rows, p.ld_x, 0, 0, kBK)))
+        return "the driver refused an operand's tensor map";
+    if (w.cg == 2) return weight_grad<256, 2>(a, b, k, w.grid, stream);
+    switch (w.bn) {
+    case 256: return weight_grad<256, 1>(a, b, k, w.grid, stream);
+    case 128: return weight_grad<128, 1>(a, b, k, w.grid, stream);
+    default: return weight_grad<64, 1>(a, b, k, w.grid, stream);
     }
-    const uint32_t n_ctas = grid ? grid : 1;
-    const dim3 join_grid(n_ctas - 1 + p.n_groups, kJoinSlices);
-    if (bn == 256) k_weight_grad_join<256><<<join_grid, kJoinThreads, 0, stream>>>(k, n_ctas);
-    else if (bn == 128) k_weight_grad_join<128><<<join_grid, kJoinThreads, 0, stream>>>(k, n_ctas);
-    else k_weight_grad_join<64><<<join_grid, kJoinThreads, 0, stream>>>(k, n_ctas);
-    return nullptr;
 }
 
 }  // namespace srf

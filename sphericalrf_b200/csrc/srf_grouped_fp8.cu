@@ -34,20 +34,33 @@ struct Fp8Args {
     unsigned int* error_flags;
 };
 
-template <int BN> __host__ __device__ constexpr int n_stages() { return BN == 256 ? 4 : BN == 128 ? 6 : 8; }
+// CG CTAs share a tile of CG*128 x BN outputs; each holds 128 rows of A and BN/CG rows of B per stage.
+template <int BN, int CG> __host__ __device__ constexpr int n_stages() { return BN / CG == 256 ? 4 : BN / CG == 128 ? 6 : 8; }
 template <int BN> __host__ __device__ constexpr int n_accs() { return BN == 256 ? 2 : 4; }
-template <int BN>
-__host__ __device__ constexpr int smem_bytes() {
-    const int b = 1024 + n_stages<BN>() * (kABytes + BN * kBK) + kStoreBytes + 512;
+template <int BN, int CG> __host__ __device__ constexpr int smem_bytes() {
+    const int b = 1024 + n_stages<BN, CG>() * (kABytes + BN / CG * kBK) + kStoreBytes + 512;
     return b < kSmemMin ? kSmemMin : b;
 }
 
-template <int BN>
+// Registers of the 256-wide tile: 128 sums and two pieces of 32 in flight per scaling thread.  The block is launched with
+// 168 a thread (64512); 128 x 64 + 256 x 216 = 63488.
+constexpr int kRegsIssue = 64, kRegsScale = 216;
+static_assert(128 * kRegsIssue + 256 * kRegsScale <= kThreads * 168, "a larger share would wait for registers forever");
+
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) { return (uint64_t)lo | (uint64_t)hi << 32; }
+// Two fused multiply-adds, each rounded once.
+__device__ __forceinline__ void fma2(uint64_t& sum, uint64_t a, uint64_t b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+
+template <int BN, int CG>
 __global__ void __launch_bounds__(kThreads, 1)
 k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Fp8Args p) {
-    constexpr int kStages = n_stages<BN>(), kAccs = n_accs<BN>();
-    constexpr int kBBytes = BN * kBK;
-    constexpr int kCols = BN / 2;                 // columns of one warpgroup
+    constexpr int kStages = n_stages<BN, CG>(), kAccs = n_accs<BN>();
+    constexpr int kBRows = BN / CG, kBBytes = kBRows * kBK;
+    constexpr int kCols = BN / 2;                 // columns of one set of scaling warps
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     unsigned char* sm_a = smem;
@@ -59,90 +72,98 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kStages;
     const uint32_t bar_acc_full = bar_empty + 8 * kStages, bar_acc_empty = bar_acc_full + 8 * kAccs;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 2 ? cluster_rank() : 0;
     const uint32_t tiles_n = (p.n_out + BN - 1) / BN;
     const uint32_t blocks_k = (p.n_in + kBK - 1) / kBK, blocks_n = (p.n_out + 127) / 128;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
-        for (int i = 0; i < kAccs; ++i) { mbar_init(bar_acc_full + 8 * i, 1); mbar_init(bar_acc_empty + 8 * i, 8); }
+        for (int i = 0; i < kStages; ++i) { mbar_init(bar_full + 8 * i, CG); mbar_init(bar_empty + 8 * i, 1); }
+        for (int i = 0; i < kAccs; ++i) { mbar_init(bar_acc_full + 8 * i, 1); mbar_init(bar_acc_empty + 8 * i, 8 * CG); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *failed = 0;
         tma_prefetch_map(&map_a);
         tma_prefetch_map(&map_b);
     }
-    if (warp == 2) tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    if (warp == 2) tmem_alloc<CG>(smem_u32(tmem_slot), kTmemCols);
     tc_fence_before();
-    __syncthreads();
+    if (CG == 2) cluster_sync(); else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
     bool bad = false, ok = true;
     GroupWalk walk;
-    uint32_t at = blockIdx.x, group = 0, tn = 0, m = 0;
+    uint32_t at = blockIdx.x / CG, group = 0, tn = 0, m = 0;
     Span span = {0, 0};
     auto next_tile = [&]() -> bool {
+        constexpr uint32_t kHeight = CG * kBM;
         uint32_t local;
         if (!walk.find(at, p.offsets, p.n_groups, p.n_rows,
-                       [&](const Span& s) { return (s.end - s.begin + kBM - 1) / kBM * tiles_n; }, &group, &span, &local, &bad))
+                       [&](const Span& s) { return (s.end - s.begin + kHeight - 1) / kHeight * tiles_n; }, &group, &span, &local, &bad))
             return false;
-        tile_place(local, (span.end - span.begin + kBM - 1) / kBM, tiles_n, &m, &tn);
-        m = span.begin + m * kBM;
-        at += gridDim.x;
+        tile_place(local, (span.end - span.begin + kHeight - 1) / kHeight, tiles_n, &m, &tn);
+        m = span.begin + m * kHeight + rank * kBM;
+        at += gridDim.x / CG;
         return true;
     };
 
-    if (warp == 0) {
-        // ---- operand loads ----
-        uint32_t s = 0, round = 0, in_flight = 0;
-        while (ok && next_tile()) {
-            for (uint32_t k = 0; k < blocks_k; ++k) {
-                if (round > 0 && !mbar_wait(bar_empty + 8 * s, (round - 1) & 1, failed)) { ok = false; break; }
-                if (elect_one()) {
-                    const uint32_t bar = bar_full + 8 * s;
-                    mbar_expect(bar, kABytes + kBBytes);
-                    tma_2d(smem_u32(sm_a) + s * kABytes, &map_a, bar, (int)(k * kBK), (int)m);
-                    tma_3d(smem_u32(sm_b) + s * kBBytes, &map_b, bar, (int)(k * kBK), (int)(tn * BN), (int)group);
+    if (warp < 4) {
+        if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsIssue));
+        if (warp == 0) {
+            // ---- operand loads ----
+            const uint32_t lead_full = CG == 2 ? leader_addr(bar_full) : bar_full;
+            uint32_t s = 0, round = 0, in_flight = 0;
+            while (ok && next_tile()) {
+                for (uint32_t k = 0; k < blocks_k; ++k) {
+                    if (round > 0 && !mbar_wait(bar_empty + 8 * s, (round - 1) & 1, failed)) { ok = false; break; }
+                    if (elect_one()) {
+                        const uint32_t bar = lead_full + 8 * s;
+                        pair_expect<CG>(bar, kABytes + kBBytes);
+                        tma_2d<CG>(smem_u32(sm_a) + s * kABytes, &map_a, bar, (int)(k * kBK), (int)m);
+                        tma_3d<CG>(smem_u32(sm_b) + s * kBBytes, &map_b, bar, (int)(k * kBK), (int)(tn * BN + rank * kBRows), (int)group);
+                    }
+                    __syncwarp();
+                    if (++s == kStages) { s = 0; ++round; }
+                    in_flight = in_flight < kStages ? in_flight + 1 : in_flight;
                 }
-                __syncwarp();
-                if (++s == kStages) { s = 0; ++round; }
-                in_flight = in_flight < kStages ? in_flight + 1 : in_flight;
             }
-        }
-        // Copies may still be on their way when another warp gave up: they must land before the CTA leaves.
-        if (!ok || *failed) {
-            for (uint32_t i = 0; i < in_flight; ++i) {
-                const uint32_t q = s >= i + 1 ? s - i - 1 : s + kStages - i - 1;
-                const uint32_t r = s >= i + 1 ? round : round - 1;
-                uint32_t none = 0;
-                mbar_wait(bar_full + 8 * q, r & 1, &none);
+            // Copies may still be on their way when another warp gave up: they must land before the CTA (or pair) leaves.
+            if ((!ok || *failed) && rank == 0) {
+                for (uint32_t i = 0; i < in_flight; ++i) {
+                    const uint32_t q = s >= i + 1 ? s - i - 1 : s + kStages - i - 1;
+                    const uint32_t r = s >= i + 1 ? round : round - 1;
+                    uint32_t none = 0;
+                    mbar_wait(bar_full + 8 * q, r & 1, &none);
+                }
             }
-        }
-    } else if (warp == 1) {
-        // ---- matrix instructions: four to a block, each block its own accumulator ----
-        constexpr uint32_t idesc = idesc_shape(BN);      // e4m3 is format 0
-        uint32_t s = 0, round = 0, acc = 0, acc_round = 0;
-        while (ok && next_tile()) {
-            for (uint32_t k = 0; k < blocks_k; ++k) {
-                if (acc_round > 0 && !mbar_wait(bar_acc_empty + 8 * acc, (acc_round - 1) & 1, failed)) { ok = false; break; }
-                if (!mbar_wait(bar_full + 8 * s, round & 1, failed)) { ok = false; break; }
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t a = smem_u32(sm_a) + s * kABytes, b = smem_u32(sm_b) + s * kBBytes;
+        } else if (warp == 1 && rank == 0) {
+            // ---- matrix instructions: four to a block, each block its own accumulator ----
+            constexpr uint32_t idesc = idesc_shape(CG * kBM, BN);      // e4m3 is format 0
+            uint32_t s = 0, round = 0, acc = 0, acc_round = 0;
+            while (ok && next_tile()) {
+                for (uint32_t k = 0; k < blocks_k; ++k) {
+                    if (acc_round > 0 && !mbar_wait(bar_acc_empty + 8 * acc, (acc_round - 1) & 1, failed)) { ok = false; break; }
+                    if (!mbar_wait(bar_full + 8 * s, round & 1, failed)) { ok = false; break; }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t a = smem_u32(sm_a) + s * kABytes, b = smem_u32(sm_b) + s * kBBytes;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        mma_f8(tmem + acc * BN, operand_desc(a + q * 32, 16, 1024), operand_desc(b + q * 32, 16, 1024), idesc, q != 0);
-                    mma_commit(bar_empty + 8 * s);
-                    mma_commit(bar_acc_full + 8 * acc);
+                        for (int q = 0; q < 4; ++q)
+                            mma_f8<CG>(tmem + acc * BN, operand_desc(a + q * 32, 16, 1024), operand_desc(b + q * 32, 16, 1024), idesc, q != 0);
+                        mma_commit<CG>(bar_empty + 8 * s);
+                        mma_commit<CG>(bar_acc_full + 8 * acc);
+                    }
+                    __syncwarp();
+                    if (++s == kStages) { s = 0; ++round; }
+                    if (++acc == kAccs) { acc = 0; ++acc_round; }
                 }
-                __syncwarp();
-                if (++s == kStages) { s = 0; ++round; }
-                if (++acc == kAccs) { acc = 0; ++acc_round; }
             }
         }
-    } else if (warp >= 4) {
+    } else {
         // ---- scale, sum, store ----
+        if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kRegsScale));
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         unsigned char* stage = sm_store + (warp - 4) * 4096;
+        const uint32_t lead_acc_empty = CG == 2 ? leader_addr(bar_acc_empty) : bar_acc_empty;
         uint32_t acc = 0, acc_round = 0;
         while (ok && next_tile()) {
             const uint32_t row0 = m + quarter * 32;
@@ -151,29 +172,35 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             const uint32_t wb = col0 / 128 < blocks_n ? col0 / 128 : blocks_n - 1;
             const float* sx = p.x_scales + row;
             const float* sw = p.w_scales + ((size_t)group * blocks_n + wb) * blocks_k;
-            float sum[kCols];
+            uint64_t sum[kCols / 2];
 #pragma unroll
-            for (int i = 0; i < kCols; ++i) sum[i] = 0.f;
+            for (int i = 0; i < kCols / 2; ++i) sum[i] = 0ull;
             float scale = __ldg(sx) * __ldg(sw);
             for (uint32_t k = 0; k < blocks_k; ++k) {
-                float ahead = 0.f;
-                if (k + 1 < blocks_k) ahead = __ldg(sx + (size_t)(k + 1) * p.n_rows) * __ldg(sw + k + 1);
+                float sx_next = 0.f, sw_next = 0.f;             // the next block's, asked for early
+                if (k + 1 < blocks_k) { sx_next = __ldg(sx + (size_t)(k + 1) * p.n_rows); sw_next = __ldg(sw + k + 1); }
+                const uint64_t scale2 = pair_of(__float_as_uint(scale), __float_as_uint(scale));
                 if (!mbar_wait(bar_acc_full + 8 * acc, acc_round & 1, failed)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t d = tmem + acc * BN + half * kCols + ((uint32_t)(quarter * 32) << 16);
+                // a piece of 32 columns is on its way while the one before it is scaled and added
+                uint32_t r[2][32];
+                tmem_ld32(d, r[0]);
 #pragma unroll
-                for (int c = 0; c < kCols; c += 32) {
-                    uint32_t r[32];
-                    tmem_ld32(d + c, r);
-                    tmem_ld_wait();
+                for (int c = 0; c < kCols / 32; ++c) {
+                    tmem_ld_wait(r[c & 1]);
+                    if (c + 1 < kCols / 32) {
+                        tmem_ld32(d + 32 * (c + 1), r[(c + 1) & 1]);
+                    } else {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) pair_arrive_read<CG>(lead_acc_empty + 8 * acc);
+                    }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[c + i] = fmaf(__uint_as_float(r[i]), scale, sum[c + i]);
+                    for (int i = 0; i < 16; ++i) fma2(sum[16 * c + i], pair_of(r[c & 1][2 * i], r[c & 1][2 * i + 1]), scale2);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar_acc_empty + 8 * acc);
                 if (++acc == kAccs) { acc = 0; ++acc_round; }
-                scale = ahead;
+                scale = sx_next * sw_next;
             }
             if (!ok) break;
             RowStore rs;
@@ -186,7 +213,7 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             unsigned char* out = p.out + row0 * p.out_row_bytes;
             if (p.relu) {
 #pragma unroll
-                for (int i = 0; i < kCols; ++i) sum[i] = relu(sum[i]);
+                for (int i = 0; i < kCols / 2; ++i) sum[i] = pair_of(__float_as_uint(relu(lo_of(sum[i]))), __float_as_uint(relu(hi_of(sum[i]))));
             }
             const uint32_t cols = col0 >= p.n_out ? 0u : p.n_out - col0 < (uint32_t)kCols ? p.n_out - col0 : (uint32_t)kCols;
             if (p.f32) {
@@ -194,9 +221,10 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 for (int c = 0; c < kCols; c += 32) {
                     if ((uint32_t)c >= cols) continue;
 #pragma unroll
-                    for (int u = 0; u < 8; ++u)
-                        stage_unit(stage, lane, u, make_uint4(__float_as_uint(sum[c + 4 * u]), __float_as_uint(sum[c + 4 * u + 1]),
-                                                              __float_as_uint(sum[c + 4 * u + 2]), __float_as_uint(sum[c + 4 * u + 3])));
+                    for (int u = 0; u < 8; ++u) {
+                        const uint64_t v0 = sum[c / 2 + 2 * u], v1 = sum[c / 2 + 2 * u + 1];
+                        stage_unit(stage, lane, u, make_uint4((uint32_t)v0, (uint32_t)(v0 >> 32), (uint32_t)v1, (uint32_t)(v1 >> 32)));
+                    }
                     rs.bytes = (cols - c < 32u ? cols - c : 32u) * 4u;
                     rs.out = out + (size_t)(col0 + c) * 4;
                     store_rows(rs, stage);
@@ -207,9 +235,12 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 for (int c = 0; c < kCols; c += kPer) {
                     if ((uint32_t)c >= cols) continue;
 #pragma unroll
-                    for (int u = 0; u < kPer / 8; ++u)
-                        stage_unit(stage, lane, u, make_uint4(pack16(sum[c + 8 * u], sum[c + 8 * u + 1], rs.bf16), pack16(sum[c + 8 * u + 2], sum[c + 8 * u + 3], rs.bf16),
-                                                              pack16(sum[c + 8 * u + 4], sum[c + 8 * u + 5], rs.bf16), pack16(sum[c + 8 * u + 6], sum[c + 8 * u + 7], rs.bf16)));
+                    for (int u = 0; u < kPer / 8; ++u) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = pack16(lo_of(sum[c / 2 + 4 * u + e]), hi_of(sum[c / 2 + 4 * u + e]), rs.bf16);
+                        stage_unit(stage, lane, u, make_uint4(w[0], w[1], w[2], w[3]));
+                    }
                     rs.bytes = (cols - c < (uint32_t)kPer ? cols - c : (uint32_t)kPer) * 2u;
                     rs.out = out + (size_t)(col0 + c) * 2;
                     store_rows(rs, stage);
@@ -219,19 +250,8 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     }
     if ((bad || (!ok && lane == 0)) && p.error_flags) atomicOr(p.error_flags, (ok ? 0u : 2u) | (bad ? 16u : 0u));
     tc_fence_before();
-    __syncthreads();
-    if (warp == 2) tmem_free(tmem, kTmemCols);
-}
-
-template <int BN>
-const char* launch(const CUtensorMap& a, const CUtensorMap& b, const Fp8Args& args, uint64_t max_units, cudaStream_t stream) {
-    static_assert(smem_bytes<BN>() <= 227 * 1024, "shared memory of one SM");
-    const int sms = sm_count();
-    if (cudaFuncSetAttribute((const void*)k_grouped_fp8<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<BN>()) != cudaSuccess)
-        return "cudaFuncSetAttribute failed";
-    const int grid = (int)(max_units < (uint64_t)sms ? max_units : (uint64_t)sms);
-    k_grouped_fp8<BN><<<grid, kThreads, smem_bytes<BN>(), stream>>>(a, b, args);
-    return nullptr;
+    if (CG == 2) cluster_sync(); else __syncthreads();      // a pair's barriers and accumulators serve both CTAs to the end
+    if (warp == 2) tmem_free<CG>(tmem, kTmemCols);
 }
 
 }  // namespace
@@ -239,15 +259,12 @@ const char* launch(const CUtensorMap& a, const CUtensorMap& b, const Fp8Args& ar
 const char* launch_grouped_matmul_fp8(const srf_grouped_t& p, const uint64_t* offsets, const void* x, const float* x_scales,
                                       const void* w, const float* w_scales, void* y, unsigned int* error_flags,
                                       cudaStream_t stream) {
-    const uint64_t busy = p.n_groups < p.n_rows ? p.n_groups : p.n_rows;
-    const uint64_t row_tiles = p.n_rows / kBM + busy;
-    if (!row_tiles) return nullptr;
-    const uint64_t want = 2ull * sm_count();
-    int bn = 256;
-    while (bn > 64 && ((uint32_t)bn / 2 >= p.n_out || row_tiles * ((p.n_out + bn - 1) / bn) < want)) bn /= 2;
+    if (!p.n_rows) return nullptr;
+    const int sms = sm_count();
+    const TileShape t = pick_tile(p, p.n_out, sms, 64);
     CUtensorMap a, b;
     if (!make_operand_map(&a, x, SRF_TYPE_E4M3, p.n_in, p.n_rows, p.ld_x, 0, 0, kBM) ||
-        !make_operand_map(&b, w, SRF_TYPE_E4M3, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, bn))
+        !make_operand_map(&b, w, SRF_TYPE_E4M3, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, t.bn / t.cg))
         return "the driver refused an operand's tensor map";
     Fp8Args k;
     memset(&k, 0, sizeof(k));
@@ -255,11 +272,12 @@ const char* launch_grouped_matmul_fp8(const srf_grouped_t& p, const uint64_t* of
     k.n_groups = p.n_groups; k.n_in = p.n_in; k.n_out = p.n_out;
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.out_type == SRF_TYPE_BF16; k.relu = p.activation == SRF_ACT_RELU;
     k.out_row_bytes = p.ld_y * (k.f32 ? 4 : 2); k.error_flags = error_flags;
-    const uint64_t units = row_tiles * ((p.n_out + bn - 1) / bn);
-    switch (bn) {
-    case 256: return launch<256>(a, b, k, units, stream);
-    case 128: return launch<128>(a, b, k, units, stream);
-    default: return launch<64>(a, b, k, units, stream);
+    const uint32_t grid = tile_grid(p, p.n_out, t, sms);
+    if (t.cg == 2) return launch_tiles(k_grouped_fp8<256, 2>, smem_bytes<256, 2>(), kThreads, 2, grid, stream, a, b, k);
+    switch (t.bn) {
+    case 256: return launch_tiles(k_grouped_fp8<256, 1>, smem_bytes<256, 1>(), kThreads, 1, grid, stream, a, b, k);
+    case 128: return launch_tiles(k_grouped_fp8<128, 1>, smem_bytes<128, 1>(), kThreads, 1, grid, stream, a, b, k);
+    default: return launch_tiles(k_grouped_fp8<64, 1>, smem_bytes<64, 1>(), kThreads, 1, grid, stream, a, b, k);
     }
 }
 

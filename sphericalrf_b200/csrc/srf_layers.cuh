@@ -30,4 +30,31 @@ bool make_operand_map(void* map, const void* base, int type, uint64_t cols, uint
                       uint64_t matrix_stride, uint32_t box_rows);
 int sm_count();
 
+// Row tiles of `height` that n_rows samples in n_groups groups can have at most.
+uint64_t max_row_tiles(const srf_grouped_t& p, uint64_t height);
+// Output tiles of a layer or an input gradient with `cols` columns: CG*128 samples x BN columns on CG CTAs.
+struct TileShape { int bn, cg; };
+TileShape pick_tile(const srf_grouped_t& p, uint32_t cols, int sms, int smallest);
+// CTAs for them: one per SM, no more than there can be tiles.
+uint32_t tile_grid(const srf_grouped_t& p, uint32_t cols, TileShape t, int sms);
+
+// One persistent launch of a tile kernel; `cg` CTAs to a cluster.
+template <class Kernel, class... Args>
+const char* launch_tiles(Kernel kernel, int smem, int threads, int cg, uint32_t grid, cudaStream_t stream, const Args&... args) {
+    if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return "cudaFuncSetAttribute failed";
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cg;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cg > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? nullptr : "the layer kernel did not launch";
+}
+
 }  // namespace srf

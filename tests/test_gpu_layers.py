@@ -151,6 +151,8 @@ SHAPES = [
     ([4096], 128, 1030, 0, 0),
     ([20000, 3], 16, 129, 0, 0),
     ([260, 900, 64, 2500], 512, 768, 0, 0),
+    ([20000, 3, 0, 18001], 136, 600, 2, 9),
+    ([9000, 30000], 700, 264, 0, 0),
 ]
 
 
