@@ -216,20 +216,23 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     Piece t;
 
     if (warp == 0) {
-        // ---- operand loads ----
+        // ---- operand loads: one thread, but for the zeroing of a group's last stage ----
         const uint32_t lead_full = CG == 2 ? leader_addr(bar_full) : bar_full;
-        uint32_t s = 0, round = 0;                     // ring position
-        uint32_t in_flight = 0, tails = 0;
+        const uint32_t a0 = smem_u32(sm_a), b0 = smem_u32(sm_b);
+        Ring<kStages> at;
+        uint32_t issued = 0, tails = 0;
         while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
             const int am = (int)(t.m + rank * kBM), bn = (int)(t.n * BN + rank * kBRows);
-            for (uint32_t k = 0; k < t.k_stages; ++k) {
-                if (round > 0 && !mbar_wait(bar_empty + 8 * s, (round - 1) & 1, failed)) { ok = false; break; }
-                const uint32_t rows = t.span.end - t.span.begin - (t.k0 + k) * kBK;      // weight gradient: samples from here on
-                const bool tail = MODE == kWeightGrad && rows < (uint32_t)kBK;
-                const uint32_t a = smem_u32(sm_a) + s * kABytes, b = smem_u32(sm_b) + s * kBBytes;
-                if (elect_one()) {
-                    const uint32_t bar = tail ? bar_tail : lead_full + 8 * s;
-                    if (tail) mbar_expect(bar_tail, kABytes + kBBytes);
+            // weight gradient: the group's last stage, if it is of this piece and not a full one
+            const uint32_t deep = t.span.end - t.span.begin;
+            const bool tail = MODE == kWeightGrad && (t.k0 + t.k_stages) * kBK > deep;
+            if (elect_one()) {
+                Ring<kStages> r = at;
+                for (uint32_t k = 0; k < t.k_stages; ++k) {
+                    if (r.round > 0 && !mbar_wait_one(bar_empty + 8 * r.slot, (r.round - 1) & 1, failed)) { ok = false; break; }
+                    const bool last = tail && k + 1 == t.k_stages;
+                    const uint32_t a = a0 + r.slot * kABytes, b = b0 + r.slot * kBBytes, bar = last ? bar_tail : lead_full + 8 * r.slot;
+                    if (last) mbar_expect(bar_tail, kABytes + kBBytes);
                     else pair_expect<CG>(bar, kABytes + kBBytes);
                     const int kk = (int)((t.k0 + k) * kBK);
                     if (kAColumns) {
@@ -247,67 +250,61 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 #pragma unroll
                         for (int i = 0; i < kBRows / 64; ++i) tma_2d<CG>(b + i * 8192, &map_b, bar, bn + 64 * i, (int)t.span.begin + kk);
                     }
+                    ++issued;
+                    r.step();
                 }
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            at.skip(t.k_stages);
+            if (tail) {
+                // When the last stage has landed, zero the next group's samples up to the next 16 (an instruction's
+                // depth), then report the stage.
+                const uint32_t q = at.slot ? at.slot - 1 : kStages - 1;
+                ok = mbar_wait(bar_tail, tails++ & 1, failed);
+                const int r0 = (int)(deep - (t.k0 + t.k_stages - 1) * kBK), r1 = (r0 + 15) & ~15;
+                zero_rows(sm_a + q * kABytes, kBM / 64, r0, r1);
+                zero_rows(sm_b + q * kBBytes, kBRows / 64, r0, r1);
+                fence_async_smem();
                 __syncwarp();
-                if (tail) {
-                    // The group's last stage: when it has landed, zero the next group's samples up to the next 16 (an
-                    // instruction's depth), then report the stage.
-                    if (!mbar_wait(bar_tail, tails++ & 1, failed)) { ok = false; break; }
-                    const int r0 = (int)rows, r1 = (r0 + 15) & ~15;
-                    zero_rows(sm_a + s * kABytes, kBM / 64, r0, r1);
-                    zero_rows(sm_b + s * kBBytes, kBRows / 64, r0, r1);
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) pair_arrive<CG>(lead_full + 8 * s);
-                    __syncwarp();
-                }
-                if (++s == kStages) { s = 0; ++round; }
-                in_flight = in_flight < kStages ? in_flight + 1 : in_flight;
+                if (lane == 0 && ok) pair_arrive<CG>(lead_full + 8 * q);
+                __syncwarp();
             }
         }
         // Copies may still be on their way when another warp gave up: they must land before the CTA (or pair) leaves.
-        if ((!ok || *failed) && rank == 0) {
-            for (uint32_t i = 0; i < in_flight; ++i) {
-                const uint32_t q = s >= i + 1 ? s - i - 1 : s + kStages - i - 1;
-                const uint32_t r = s >= i + 1 ? round : round - 1;
-                uint32_t none = 0;
-                mbar_wait(bar_full + 8 * q, r & 1, &none);
-            }
-        }
+        if ((!ok || *failed) && rank == 0) drain_ring<kStages>(bar_full, issued);
     } else if (warp == 1 && rank == 0) {
-        // ---- matrix instructions ----
+        // ---- matrix instructions: one thread ----
         const uint32_t idesc = idesc_shape(CG * kBM, BN) | (p.bf16 ? (1u << 7) | (1u << 10) : 0u) | (kAColumns ? 1u << 15 : 0u) | (kBColumns ? 1u << 16 : 0u);
-        uint32_t s = 0, round = 0, acc = 0, acc_round = 0;
+        const uint64_t desc_a = operand_desc(smem_u32(sm_a), kAColumns ? 8192 : 16, 1024), desc_b = operand_desc(smem_u32(sm_b), kBColumns ? 8192 : 16, 1024);
+        constexpr uint32_t kStepA = kAColumns ? 2048 : 32, kStepB = kBColumns ? 2048 : 32;      // bytes of 16 summed indices
+        Ring<kStages> at;
+        Ring<kAccs> acc;
         while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
-            if (acc_round > 0 && !mbar_wait(bar_acc_empty + 8 * acc, (acc_round - 1) & 1, failed)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t d = tmem + acc * BN;
-            for (uint32_t k = 0; k < t.k_stages; ++k) {
-                if (!mbar_wait(bar_full + 8 * s, round & 1, failed)) { ok = false; break; }
-                tc_fence_after();
-                int k_steps = kBK / 16;
-                if (MODE == kWeightGrad) {
-                    const uint32_t rows = t.span.end - t.span.begin - (t.k0 + k) * kBK;
-                    if (rows < (uint32_t)kBK) {
-                        k_steps = (int)(rows + 15) / 16;
+            if (elect_one()) {
+                Ring<kStages> r = at;
+                const uint32_t d = tmem + acc.slot * BN, deep = t.span.end - t.span.begin;
+                if (acc.round > 0) ok = mbar_wait_one(bar_acc_empty + 8 * acc.slot, (acc.round - 1) & 1, failed);
+                for (uint32_t k = 0; ok && k < t.k_stages; ++k) {
+                    if (!mbar_wait_one(bar_full + 8 * r.slot, r.round & 1, failed)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t da = desc_at(desc_a, r.slot * kABytes), db = desc_at(desc_b, r.slot * kBBytes);
+                    const uint32_t rows = deep - (t.k0 + k) * kBK;
+                    if (MODE == kWeightGrad && rows < (uint32_t)kBK) {
                         pair_acquire<CG>();                // the other CTA zeroed rows of its operands
+                        for (uint32_t q = 0; q < (rows + 15) / 16; ++q) mma_f16<CG>(d, desc_at(da, q * kStepA), desc_at(db, q * kStepB), idesc, (k | q) != 0);
+                    } else {
+#pragma unroll
+                        for (uint32_t q = 0; q < kBK / 16; ++q) mma_f16<CG>(d, desc_at(da, q * kStepA), desc_at(db, q * kStepB), idesc, (k | q) != 0);
                     }
+                    mma_commit<CG>(bar_empty + 8 * r.slot);
+                    r.step();
                 }
-                if (elect_one()) {
-                    const uint32_t a = smem_u32(sm_a) + s * kABytes, b = smem_u32(sm_b) + s * kBBytes;
-                    for (int q = 0; q < k_steps; ++q) {
-                        const uint64_t da = kAColumns ? operand_desc(a + q * 2048, 8192, 1024) : operand_desc(a + q * 32, 16, 1024);
-                        const uint64_t db = kBColumns ? operand_desc(b + q * 2048, 8192, 1024) : operand_desc(b + q * 32, 16, 1024);
-                        mma_f16<CG>(d, da, db, idesc, (k | (uint32_t)q) != 0);
-                    }
-                    mma_commit<CG>(bar_empty + 8 * s);
-                    if (k + 1 == t.k_stages) mma_commit<CG>(bar_acc_full + 8 * acc);
-                }
-                __syncwarp();
-                if (++s == kStages) { s = 0; ++round; }
+                if (ok) mma_commit<CG>(bar_acc_full + 8 * acc.slot);
             }
-            if (!ok) break;
-            if (++acc == kAccs) { acc = 0; ++acc_round; }
+            ok = __all_sync(0xffffffffu, ok);
+            at.skip(t.k_stages);
+            acc.step();
         }
     } else if (warp >= 4) {
         // ---- finished accumulators to memory ----

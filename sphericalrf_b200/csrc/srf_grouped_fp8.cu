@@ -109,53 +109,56 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     if (warp < 4) {
         if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsIssue));
         if (warp == 0) {
-            // ---- operand loads ----
+            // ---- operand loads: one thread ----
             const uint32_t lead_full = CG == 2 ? leader_addr(bar_full) : bar_full;
-            uint32_t s = 0, round = 0, in_flight = 0;
+            const uint32_t a0 = smem_u32(sm_a), b0 = smem_u32(sm_b);
+            Ring<kStages> at_stage;
+            uint32_t issued = 0;
             while (ok && next_tile()) {
-                for (uint32_t k = 0; k < blocks_k; ++k) {
-                    if (round > 0 && !mbar_wait(bar_empty + 8 * s, (round - 1) & 1, failed)) { ok = false; break; }
-                    if (elect_one()) {
-                        const uint32_t bar = lead_full + 8 * s;
+                if (elect_one()) {
+                    Ring<kStages> r = at_stage;
+                    for (uint32_t k = 0; k < blocks_k; ++k) {
+                        if (r.round > 0 && !mbar_wait_one(bar_empty + 8 * r.slot, (r.round - 1) & 1, failed)) { ok = false; break; }
+                        const uint32_t bar = lead_full + 8 * r.slot;
                         pair_expect<CG>(bar, kABytes + kBBytes);
-                        tma_2d<CG>(smem_u32(sm_a) + s * kABytes, &map_a, bar, (int)(k * kBK), (int)m);
-                        tma_3d<CG>(smem_u32(sm_b) + s * kBBytes, &map_b, bar, (int)(k * kBK), (int)(tn * BN + rank * kBRows), (int)group);
+                        tma_2d<CG>(a0 + r.slot * kABytes, &map_a, bar, (int)(k * kBK), (int)m);
+                        tma_3d<CG>(b0 + r.slot * kBBytes, &map_b, bar, (int)(k * kBK), (int)(tn * BN + rank * kBRows), (int)group);
+                        ++issued;
+                        r.step();
                     }
-                    __syncwarp();
-                    if (++s == kStages) { s = 0; ++round; }
-                    in_flight = in_flight < kStages ? in_flight + 1 : in_flight;
                 }
+                ok = __all_sync(0xffffffffu, ok);
+                at_stage.skip(blocks_k);
             }
             // Copies may still be on their way when another warp gave up: they must land before the CTA (or pair) leaves.
-            if ((!ok || *failed) && rank == 0) {
-                for (uint32_t i = 0; i < in_flight; ++i) {
-                    const uint32_t q = s >= i + 1 ? s - i - 1 : s + kStages - i - 1;
-                    const uint32_t r = s >= i + 1 ? round : round - 1;
-                    uint32_t none = 0;
-                    mbar_wait(bar_full + 8 * q, r & 1, &none);
-                }
-            }
+            if ((!ok || *failed) && rank == 0) drain_ring<kStages>(bar_full, issued);
         } else if (warp == 1 && rank == 0) {
-            // ---- matrix instructions: four to a block, each block its own accumulator ----
+            // ---- matrix instructions: one thread; four to a block, each block its own accumulator ----
             constexpr uint32_t idesc = idesc_shape(CG * kBM, BN);      // e4m3 is format 0
-            uint32_t s = 0, round = 0, acc = 0, acc_round = 0;
+            const uint64_t desc_a = operand_desc(smem_u32(sm_a), 16, 1024), desc_b = operand_desc(smem_u32(sm_b), 16, 1024);
+            Ring<kStages> at_stage;
+            Ring<kAccs> at_acc;
             while (ok && next_tile()) {
-                for (uint32_t k = 0; k < blocks_k; ++k) {
-                    if (acc_round > 0 && !mbar_wait(bar_acc_empty + 8 * acc, (acc_round - 1) & 1, failed)) { ok = false; break; }
-                    if (!mbar_wait(bar_full + 8 * s, round & 1, failed)) { ok = false; break; }
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint32_t a = smem_u32(sm_a) + s * kABytes, b = smem_u32(sm_b) + s * kBBytes;
+                if (elect_one()) {
+                    Ring<kStages> r = at_stage;
+                    Ring<kAccs> acc = at_acc;
+                    for (uint32_t k = 0; k < blocks_k; ++k) {
+                        if (acc.round > 0 && !mbar_wait_one(bar_acc_empty + 8 * acc.slot, (acc.round - 1) & 1, failed)) { ok = false; break; }
+                        if (!mbar_wait_one(bar_full + 8 * r.slot, r.round & 1, failed)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint64_t da = desc_at(desc_a, r.slot * kABytes), db = desc_at(desc_b, r.slot * kBBytes);
+                        const uint32_t d = tmem + acc.slot * BN;
 #pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            mma_f8<CG>(tmem + acc * BN, operand_desc(a + q * 32, 16, 1024), operand_desc(b + q * 32, 16, 1024), idesc, q != 0);
-                        mma_commit<CG>(bar_empty + 8 * s);
-                        mma_commit<CG>(bar_acc_full + 8 * acc);
+                        for (uint32_t q = 0; q < 4; ++q) mma_f8<CG>(d, desc_at(da, q * 32), desc_at(db, q * 32), idesc, q != 0);
+                        mma_commit<CG>(bar_acc_full + 8 * acc.slot);
+                        mma_commit<CG>(bar_empty + 8 * r.slot);
+                        r.step();
+                        acc.step();
                     }
-                    __syncwarp();
-                    if (++s == kStages) { s = 0; ++round; }
-                    if (++acc == kAccs) { acc = 0; ++acc_round; }
                 }
+                ok = __all_sync(0xffffffffu, ok);
+                at_stage.skip(blocks_k);
+                at_acc.skip(blocks_k);
             }
         }
     } else {

@@ -37,26 +37,43 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
 // accumulation of one output tile over 2^26 rows, well under a second.
 constexpr long long kWaitCycles = 8000000000ll;
 
-// Bounded wait of a whole warp, with one answer for all its lanes.  `failed` (shared memory) tells the CTA's other warps
-// that one of them gave up.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
-    long long t0 = 0;
-    for (uint32_t i = 0; i < (1u << 26); ++i) {
-#pragma unroll 1
-        for (int q = 0; q < 64; ++q)
-            if (__any_sync(0xffffffffu, mbar_test(bar, parity))) return true;
-        if (i == 0) t0 = clock64();
-        if (__any_sync(0xffffffffu, *failed != 0 || clock64() - t0 > kWaitCycles)) break;
+// Bounded wait of one thread.  `failed` (shared memory) tells the CTA's other warps that one of them gave up.
+__device__ __forceinline__ bool mbar_wait_one(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
+    if (mbar_test(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (uint32_t i = 1; i < (1u << 31); ++i) {
+        if (mbar_test(bar, parity)) return true;
+        if ((i & 63u) == 0 && (*failed != 0 || clock64() - t0 > kWaitCycles)) break;
     }
     *failed = 1;
     return false;
 }
+// The same for a whole warp, with one answer for all its lanes: a phase that one lane saw complete is complete.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
+    if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+    const bool done = mbar_wait_one(bar, parity, failed);
+    return __any_sync(0xffffffffu, done);
+}
 
+// One lane of a converged warp, the same one every time.  The compiler knows that a single thread is behind it, which the
+// instructions with uniform operands (TMA, tcgen05) are issued faster for than behind `lane == 0`.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
     return p != 0;
 }
+
+// Place in a ring of `N` slots, advanced by all lanes of a warp alike.
+template <int N>
+struct Ring {
+    uint32_t slot = 0, round = 0;
+    __device__ __forceinline__ void step() { if (++slot == N) { slot = 0; ++round; } }
+    __device__ __forceinline__ void skip(uint32_t n) {
+        const uint32_t to = slot + n, turns = to / N;
+        round += turns;
+        slot = to - turns * N;
+    }
+};
 
 // ---- pairs of CTAs (CG = 2): two SMs work on one tile, the CTA of rank 0 issues for both ----
 
@@ -135,6 +152,9 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t lbo, ui
            (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
+// The same operand `bytes` further on (a multiple of 16; the address field does not overflow inside shared memory).
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
+
 template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     if (CG == 1)
@@ -162,6 +182,17 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
         asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                      :: "r"(bar), "h"((uint16_t)3) : "memory");
 }
+// Waits (bounded) for the copies of a ring's last stages that nobody else will wait for; one warp of rank 0.
+template <int N>
+__device__ __forceinline__ void drain_ring(uint32_t bar_full, uint32_t issued) {
+    issued = __reduce_max_sync(0xffffffffu, issued);
+    for (uint32_t i = 0; i < issued && i < N; ++i) {
+        const uint32_t q = issued - 1 - i;
+        uint32_t none = 0;
+        mbar_wait(bar_full + 8 * (q % N), (q / N) & 1, &none);
+    }
+}
+
 template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols) {
     if (CG == 1) {
@@ -284,7 +315,10 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
     return r;
 }
 // NaN stays NaN.
-__device__ __forceinline__ float relu(float v) { return v < 0.f ? 0.f : v; }
+__device__ __forceinline__ float relu(float v) {
+    asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(v));
+    return v;
+}
 
 // x > 0 for a 16-bit value of either type: sign clear, not zero, not NaN.
 __device__ __forceinline__ bool positive16(uint32_t h, bool bf16) {
