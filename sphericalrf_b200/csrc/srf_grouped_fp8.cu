@@ -20,7 +20,9 @@ constexpr int kThreads = 384;                 // TMA, MMA, TMEM owner, spare, 8 
 constexpr int kBM = 128, kBK = 128;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kABytes = kBM * kBK;
-constexpr int kStoreBytes = 8 * 4096;
+constexpr int kStoreBytes = 8 * 4096;         // staging of the scaling warps
+constexpr int kScaleAhead = 4;                // blocks whose scales are on their way
+constexpr int kScaleBytes = 8 * kScaleAhead * 128;
 constexpr int kSmemMin = 120 * 1024;          // a second CTA that allocates TMEM must never share the SM
 
 struct Fp8Args {
@@ -35,10 +37,10 @@ struct Fp8Args {
 };
 
 // CG CTAs share a tile of CG*128 x BN outputs; each holds 128 rows of A and BN/CG rows of B per stage.
-template <int BN, int CG> __host__ __device__ constexpr int n_stages() { return BN / CG == 256 ? 4 : BN / CG == 128 ? 6 : 8; }
+template <int BN, int CG> __host__ __device__ constexpr int n_stages() { return BN / CG == 256 ? 3 : BN / CG == 128 ? 5 : 7; }
 template <int BN> __host__ __device__ constexpr int n_accs() { return BN == 256 ? 2 : 4; }
 template <int BN, int CG> __host__ __device__ constexpr int smem_bytes() {
-    const int b = 1024 + n_stages<BN, CG>() * (kABytes + BN / CG * kBK) + kStoreBytes + 512;
+    const int b = 1024 + n_stages<BN, CG>() * (kABytes + BN / CG * kBK) + kStoreBytes + kScaleBytes + 512;
     return b < kSmemMin ? kSmemMin : b;
 }
 
@@ -55,6 +57,14 @@ __device__ __forceinline__ void fma2(uint64_t& sum, uint64_t a, uint64_t b) {
 __device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
 __device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 
+// Copies of one lane's own values into shared memory, in groups that complete in order.
+__device__ __forceinline__ void copy_async4(float* dst, const float* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
 template <int BN, int CG>
 __global__ void __launch_bounds__(kThreads, 1)
 k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Fp8Args p) {
@@ -66,7 +76,8 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     unsigned char* sm_a = smem;
     unsigned char* sm_b = smem + kStages * kABytes;
     unsigned char* sm_store = sm_b + kStages * kBBytes;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sm_store + kStoreBytes);
+    float* sm_scale = reinterpret_cast<float*>(sm_store + kStoreBytes);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm_store + kStoreBytes + kScaleBytes);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2 * kAccs);
     volatile uint32_t* failed = tmem_slot + 1;
     const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kStages;
@@ -178,10 +189,26 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             uint64_t sum[kCols / 2];
 #pragma unroll
             for (int i = 0; i < kCols / 2; ++i) sum[i] = 0ull;
-            float scale = __ldg(sx) * __ldg(sw);
+            // The sample's scales come through a ring in shared memory, every lane its own, four blocks ahead, and the matrix's one
+            // per lane, 32 blocks at a time.  (Loaded into registers one block ahead, 250 of 920 cycles a block went into
+            // waiting for L2; further ahead, the registers spilled.)
+            float* ring = sm_scale + (warp - 4) * (kScaleAhead * 32) + lane;
+            const float* sx_ahead = sx;
+#pragma unroll
+            for (uint32_t u = 0; u < kScaleAhead; ++u) {
+                if (u < blocks_k) copy_async4(ring + u * 32, sx_ahead);
+                copy_async_group();
+                sx_ahead += p.n_rows;
+            }
+            float sw_lane = 0.f;
             for (uint32_t k = 0; k < blocks_k; ++k) {
-                float sx_next = 0.f, sw_next = 0.f;             // the next block's, asked for early
-                if (k + 1 < blocks_k) { sx_next = __ldg(sx + (size_t)(k + 1) * p.n_rows); sw_next = __ldg(sw + k + 1); }
+                if ((k & 31) == 0) sw_lane = k + lane < blocks_k ? __ldg(sw + k + lane) : 0.f;
+                copy_async_wait<kScaleAhead - 1>();
+                float* slot = ring + (k % kScaleAhead) * 32;
+                const float scale = *slot * __shfl_sync(0xffffffffu, sw_lane, k & 31);
+                if (k + kScaleAhead < blocks_k) copy_async4(slot, sx_ahead);
+                copy_async_group();
+                sx_ahead += p.n_rows;
                 const uint64_t scale2 = pair_of(__float_as_uint(scale), __float_as_uint(scale));
                 if (!mbar_wait(bar_acc_full + 8 * acc, acc_round & 1, failed)) { ok = false; break; }
                 tc_fence_after();
@@ -203,7 +230,6 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     for (int i = 0; i < 16; ++i) fma2(sum[16 * c + i], pair_of(r[c & 1][2 * i], r[c & 1][2 * i + 1]), scale2);
                 }
                 if (++acc == kAccs) { acc = 0; ++acc_round; }
-                scale = sx_next * sw_next;
             }
             if (!ok) break;
             RowStore rs;
