@@ -1061,8 +1061,7 @@ srf_status srf_quantize_rows(srf_ctx* ctx, int type, uint64_t n_rows, const uint
     const std::string why = refuse_quantize_rows(type, n_rows, d_n_rows_used, n_cols, d_in, &ld_in, d_out, &ld_out, d_scales);
     if (!why.empty()) return fail(ctx, SRF_ERR_ARG, why);
     DeviceGuard guard(ctx->device);
-    launch_quantize_rows(type, n_rows, d_n_rows_used, n_cols, d_in, ld_in, d_out, ld_out, d_scales, (cudaStream_t)stream);
-    return launched(ctx, nullptr);
+    return launched(ctx, launch_quantize_rows(type, n_rows, d_n_rows_used, n_cols, d_in, ld_in, d_out, ld_out, d_scales, (cudaStream_t)stream));
 }
 
 srf_status srf_quantize_weights(srf_ctx* ctx, int type, uint32_t n_matrices, uint32_t n_rows, uint32_t n_cols, const void* d_in,
@@ -1071,8 +1070,8 @@ srf_status srf_quantize_weights(srf_ctx* ctx, int type, uint32_t n_matrices, uin
     const std::string why = refuse_quantize_weights(type, n_matrices, n_rows, n_cols, d_in, &ld_in, d_out, &ld_out, d_scales);
     if (!why.empty()) return fail(ctx, SRF_ERR_ARG, why);
     DeviceGuard guard(ctx->device);
-    launch_quantize_weights(type, n_matrices, n_rows, n_cols, d_in, ld_in, n_rows * ld_in, d_out, ld_out, n_rows * ld_out, d_scales, (cudaStream_t)stream);
-    return launched(ctx, nullptr);
+    return launched(ctx, launch_quantize_weights(type, n_matrices, n_rows, n_cols, d_in, ld_in, n_rows * ld_in, d_out, ld_out, n_rows * ld_out,
+                                                 d_scales, (cudaStream_t)stream));
 }
 
 srf_status srf_volume_rendering(srf_ctx* ctx, const srf_view_t* view, const uint64_t* d_offsets, uint64_t n_rays,

@@ -208,6 +208,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if (CG == 2) cluster_sync(); else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    wait_for_inputs();
+    let_next_start();
 
     bool bad = false, ok = true;
     Pieces<MODE, CG> pieces;
@@ -226,20 +228,25 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             // weight gradient: the group's last stage, if it is of this piece and not a full one
             const uint32_t deep = t.span.end - t.span.begin;
             const bool tail = MODE == kWeightGrad && (t.k0 + t.k_stages) * kBK > deep;
+            // single CTAs load only the rows that the group has (what lies in the others' place is never stored)
+            const uint32_t boxes = MODE == kWeightGrad || CG == 2 || t.span.end - t.m >= (uint32_t)kBM ? kBM / kRowBox : (t.span.end - t.m + kRowBox - 1) / kRowBox;
+            const uint32_t bytes = boxes * (kABytes / (kBM / kRowBox)) + kBBytes;
             if (elect_one()) {
                 Ring<kStages> r = at;
                 for (uint32_t k = 0; k < t.k_stages; ++k) {
                     if (r.round > 0 && !mbar_wait_one(bar_empty + 8 * r.slot, (r.round - 1) & 1, failed)) { ok = false; break; }
                     const bool last = tail && k + 1 == t.k_stages;
                     const uint32_t a = a0 + r.slot * kABytes, b = b0 + r.slot * kBBytes, bar = last ? bar_tail : lead_full + 8 * r.slot;
-                    if (last) mbar_expect(bar_tail, kABytes + kBBytes);
-                    else pair_expect<CG>(bar, kABytes + kBBytes);
+                    if (last) mbar_expect(bar_tail, bytes);
+                    else pair_expect<CG>(bar, bytes);
                     const int kk = (int)((t.k0 + k) * kBK);
                     if (kAColumns) {
 #pragma unroll
                         for (int i = 0; i < kBM / 64; ++i) tma_2d<CG>(a + i * 8192, &map_a, bar, am + 64 * i, (int)t.span.begin + kk);
-                    } else {
+                    } else if (CG == 2) {
                         tma_2d<CG>(a, &map_a, bar, kk, am);
+                    } else {
+                        for (uint32_t i = 0; i < boxes; ++i) tma_2d<CG>(a + i * (kRowBox * 128), &map_a, bar, kk, am + (int)(i * kRowBox));
                     }
                     if (MODE == kLayer) {
                         tma_3d<CG>(b, &map_b, bar, kk, bn, (int)t.group);
@@ -401,19 +408,25 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if (warp == 2) tmem_free<CG>(tmem, kTmemCols);
 }
 
-// Second kernel of the weight gradient.  Blocks (v, slice) with v < n_workers - 1: the boundary behind worker v.  If it
-// cuts an output tile and is the first to cut it, sums the tile's partial sums in the workers' order (the slice: a few of
-// its rows).  The other blocks (n_workers - 1 + g, slice) write the zeros of a group without samples.
+// Second kernel of the weight gradient: sums the partial sums of every output tile that a boundary between two workers
+// cuts, in a fixed order of the workers, and writes the zeros of groups without samples.  A block takes a slice of a tile:
+// LANES threads share a quad of sums, each taking every LANES-th worker.
+//
+// BY_TILE: blocks (tile, slice).  Otherwise, where there are more tiles than boundaries, blocks (v, slice) with v <
+// n_workers - 1 for the boundary behind worker v, which take the tile when this boundary is the first to cut it, and
+// blocks (n_workers - 1 + g, slice) for the zeros of group g.
 constexpr int kJoinThreads = 256;
-template <int BN, int CG> __host__ __device__ constexpr int join_slices() { return CG * BN / 16; }      // 2048 sums a block
+template <int BN, int CG, int LANES> __host__ __device__ constexpr int join_slices() { return CG * kBM * BN / 4 / (LANES == 1 ? 512 : kJoinThreads / LANES); }
 
-template <int BN, int CG>
+template <int BN, int CG, int LANES, bool BY_TILE>
 __global__ void __launch_bounds__(kJoinThreads) k_weight_grad_join(const GroupedArgs p) {
-    constexpr uint32_t kSlices = join_slices<BN, CG>(), kRows = CG * kBM / kSlices, kQuads = kRows * BN / 4;
+    constexpr uint32_t kSlices = join_slices<BN, CG, LANES>(), kQuads = CG * kBM * BN / 4 / kSlices;
     const uint32_t tiles_n = (p.out_cols + BN - 1) / BN, tiles_m = (p.out_rows + CG * kBM - 1) / (CG * kBM);
     const uint32_t across = tiles_m * tiles_n, slice = blockIdx.y, n = p.n_workers;
+    wait_for_inputs();
+    let_next_start();
     bool bad = false;
-    if (blockIdx.x >= n - 1) {
+    if (!BY_TILE && blockIdx.x >= n - 1) {
         const uint32_t g = blockIdx.x - (n - 1);
         const Span s = group_span(p.offsets, g, p.n_rows, &bad);
         if (s.end > s.begin) return;
@@ -426,42 +439,76 @@ __global__ void __launch_bounds__(kJoinThreads) k_weight_grad_join(const Grouped
         }
         return;
     }
-    __shared__ uint32_t sh[5];         // first and last worker of the tile, its group, m, n
+    __shared__ uint32_t sh[6];         // first and last worker of the tile, its group, m, n; no samples
     if (threadIdx.x < 32) {
-        const uint32_t units = all_units<kWeightGrad, CG>(p, across, &bad);
-        const uint32_t u = first_unit(units, blockIdx.x + 1, n);       // first unit behind the boundary
-        GroupWalk walk;
-        uint32_t group = 0, local = 0, v0 = 1, v1 = 0, tm = 0, tn = 0;
-        Span s = {0, 0};
-        if (u > 0 && u < units &&
-            walk.find(u, p.offsets, p.n_groups, p.n_rows, [&](const Span& q) { return group_units<kWeightGrad, CG>(q, across); }, &group, &s, &local, &bad)) {
-            const uint32_t deep = (s.end - s.begin + kBK - 1) / kBK, t = local / deep, k = local - t * deep;
-            const uint32_t u0 = u - k, before = first_unit(units, blockIdx.x, n);
-            // the boundary cuts the tile, and the one in front of it does not
-            if (k > 0 && before <= u0 && before < u) {
-                v0 = blockIdx.x;
-                v1 = v0 + 1;
-                while (v1 + 1 < n && first_unit(units, v1 + 1, n) < u0 + deep) ++v1;
-                tile_place(t, tiles_m, tiles_n, &tm, &tn);
+        auto units_of = [&](const Span& q) { return group_units<kWeightGrad, CG>(q, across); };
+        uint32_t group = 0, local = 0, v0 = 1, v1 = 0, tm = 0, tn = 0, empty = 0;
+        if (BY_TILE) {
+            // units of all groups, and of those in front of this one
+            group = blockIdx.x / across;
+            uint32_t all = 0, before = 0;
+            for (uint32_t g = threadIdx.x; g < p.n_groups; g += 32) {
+                const uint32_t u = units_of(group_span(p.offsets, g, p.n_rows, &bad));
+                all += u;
+                before += g < group ? u : 0;
+            }
+            all = __reduce_add_sync(0xffffffffu, all);
+            before = __reduce_add_sync(0xffffffffu, before);
+            const Span s = group_span(p.offsets, group, p.n_rows, &bad);
+            const uint32_t t = blockIdx.x - group * across, deep = (s.end - s.begin + kBK - 1) / kBK;
+            tile_place(t, tiles_m, tiles_n, &tm, &tn);
+            if (!deep) {
+                empty = 1;
+            } else {
+                const uint32_t q = all / n, r = all - q * n;
+                auto owner = [&](uint32_t u) { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; };
+                const uint32_t u0 = before + t * deep, a = owner(u0), b = owner(u0 + deep - 1);
+                if (a < b) { v0 = a; v1 = b; }
+            }
+        } else {
+            const uint32_t units = all_units<kWeightGrad, CG>(p, across, &bad);
+            const uint32_t u = first_unit(units, blockIdx.x + 1, n);       // first unit behind the boundary
+            GroupWalk walk;
+            Span s = {0, 0};
+            if (u > 0 && u < units && walk.find(u, p.offsets, p.n_groups, p.n_rows, units_of, &group, &s, &local, &bad)) {
+                const uint32_t deep = (s.end - s.begin + kBK - 1) / kBK, t = local / deep, k = local - t * deep;
+                const uint32_t u0 = u - k, before = first_unit(units, blockIdx.x, n);
+                // the boundary cuts the tile, and the one in front of it does not
+                if (k > 0 && before <= u0 && before < u) {
+                    v0 = blockIdx.x;
+                    v1 = v0 + 1;
+                    while (v1 + 1 < n && first_unit(units, v1 + 1, n) < u0 + deep) ++v1;
+                    tile_place(t, tiles_m, tiles_n, &tm, &tn);
+                }
             }
         }
-        if (threadIdx.x == 0) { sh[0] = v0; sh[1] = v1; sh[2] = group; sh[3] = tm; sh[4] = tn; }
+        if (threadIdx.x == 0) { sh[0] = v0; sh[1] = v1; sh[2] = group; sh[3] = tm; sh[4] = tn; sh[5] = empty; }
     }
     __syncthreads();
-    const uint32_t v0 = sh[0], v1 = sh[1];
-    if (v0 > v1) return;
-    for (uint32_t i = threadIdx.x; i < kQuads; i += kJoinThreads) {
-        const uint32_t row = slice * kRows + i / (BN / 4), col = i % (BN / 4) * 4;
+    const uint32_t v0 = sh[0], v1 = sh[1], empty = sh[5], part = threadIdx.x % LANES;
+    if (v0 > v1 && !empty) return;
+    for (uint32_t i = threadIdx.x / LANES; i < kQuads; i += kJoinThreads / LANES) {
+        const uint32_t at = slice * kQuads + i, row = at / (BN / 4), col = at % (BN / 4) * 4;
         const uint32_t orow = sh[3] * (CG * kBM) + row, ocol = sh[4] * BN + col;
-        if (orow >= p.out_rows || ocol >= p.out_cols) continue;
-        const float4* q = reinterpret_cast<const float4*>(p.partial + (size_t)row * BN + col);
-        constexpr size_t kSlot = (size_t)CG * kBM * BN / 4;
-        float4 sum = q[(2 * (size_t)v0 + 1) * kSlot];
-#pragma unroll 8
-        for (uint32_t v = v0 + 1; v <= v1; ++v) {
-            const float4 e = q[2 * (size_t)v * kSlot];
-            sum.x += e.x; sum.y += e.y; sum.z += e.z; sum.w += e.w;
+        const bool inside = orow < p.out_rows && ocol < p.out_cols;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (inside && !empty) {
+            const float4* q = reinterpret_cast<const float4*>(p.partial + (size_t)row * BN + col);
+            constexpr size_t kSlot = (size_t)CG * kBM * BN / 4;
+#pragma unroll 4
+            for (uint32_t v = v0 + part; v <= v1; v += LANES) {
+                const float4 e = q[(2 * (size_t)v + (v == v0 ? 1 : 0)) * kSlot];
+                sum.x += e.x; sum.y += e.y; sum.z += e.z; sum.w += e.w;
+            }
         }
+#pragma unroll
+        for (int d = LANES / 2; d; d >>= 1) {
+            sum.x += __shfl_xor_sync(0xffffffffu, sum.x, d);
+            sum.y += __shfl_xor_sync(0xffffffffu, sum.y, d);
+            sum.z += __shfl_xor_sync(0xffffffffu, sum.z, d);
+            sum.w += __shfl_xor_sync(0xffffffffu, sum.w, d);
+        }
+        if (!inside || part) continue;
         unsigned char* o = p.out + sh[2] * p.out_group_bytes + orow * p.out_row_bytes;
         const float f[4] = {sum.x, sum.y, sum.z, sum.w};
         if (p.f32 && ocol + 4 <= p.out_cols) {
@@ -500,7 +547,7 @@ WeightGradPlan plan_weight_grad(const srf_grouped_t& p, int sms) {
 template <int MODE, int BN, int CG>
 const char* launch(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& args, uint32_t grid, cudaStream_t stream) {
     static_assert(smem_bytes<BN, CG>() <= 227 * 1024, "shared memory of one SM");
-    return launch_tiles(k_grouped<MODE, BN, CG>, smem_bytes<BN, CG>(), kThreads, CG, grid, stream, a, b, args);
+    return launch_layer(k_grouped<MODE, BN, CG>, smem_bytes<BN, CG>(), kThreads, CG, dim3(grid), stream, a, b, args);
 }
 
 }  // namespace
@@ -513,12 +560,20 @@ uint64_t max_row_tiles(const srf_grouped_t& p, uint64_t height) {
 TileShape pick_tile(const srf_grouped_t& p, uint32_t cols, int sms, int smallest) {
     // Pairs: groups of a few 256-row tiles at least, and enough tiles for every pair.
     if (cols > 128 && p.n_rows / p.n_groups >= 512 && p.n_rows / 256 * ((cols + 255) / 256) >= (uint64_t)sms) return {256, 2};
-    // Otherwise the widest tile that leaves every SM a few (a wide tile reads its operands from L2 less often, a
-    // narrow one spreads few tiles over more SMs).
-    const uint64_t row_tiles = max_row_tiles(p, 128);
-    int bn = 256;
-    while (bn > smallest && ((uint32_t)bn / 2 >= cols || row_tiles * ((cols + bn - 1) / bn) < 2ull * sms)) bn /= 2;
-    return {bn, 1};
+    // Otherwise the width that costs least: rounds of tiles over the SMs, times a tile's share of loads -- its columns, its
+    // samples, and as much as 32 columns for what every tile costs.
+    const uint64_t busy = p.n_groups < p.n_rows ? p.n_groups : p.n_rows;
+    const uint64_t mean = (p.n_rows + busy - 1) / busy;
+    const uint64_t row_tiles = mean <= 128 ? busy : p.n_rows / 128 + busy / 2;
+    int best = smallest;
+    uint64_t least = ~0ull;
+    for (int bn = smallest; bn <= 256; bn *= 2) {
+        const uint64_t tiles = row_tiles * ((cols + bn - 1) / bn);
+        const uint64_t cost = (tiles + sms - 1) / sms * (bn + (mean < 128 ? mean : 128) + 32);
+        if (cost <= least) { least = cost; best = bn; }
+        if ((uint32_t)bn >= cols) break;
+    }
+    return {best, 1};
 }
 
 uint32_t tile_grid(const srf_grouped_t& p, uint32_t cols, TileShape t, int sms) {
@@ -563,7 +618,7 @@ const char* launch_grouped_matmul(const srf_grouped_t& p, const uint64_t* offset
     const int sms = sm_count();
     const TileShape t = pick_tile(p, p.n_out, sms, 32);
     CUtensorMap a, b;
-    if (!make_operand_map(&a, x, p.type, p.n_in, p.n_rows, p.ld_x, 0, 0, kBM) ||
+    if (!make_operand_map(&a, x, p.type, p.n_in, p.n_rows, p.ld_x, 0, 0, t.cg == 2 ? kBM : kRowBox) ||
         !make_operand_map(&b, w, p.type, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, t.bn / t.cg))
         return "the driver refused an operand's tensor map";
     GroupedArgs k;
@@ -587,7 +642,7 @@ const char* launch_grouped_input_grad(const srf_grouped_t& p, const uint64_t* of
     const int sms = sm_count();
     const TileShape t = pick_tile(p, p.n_in, sms, 64);
     CUtensorMap a, b;
-    if (!make_operand_map(&a, dy, p.type, p.n_out, p.n_rows, p.ld_y, 0, 0, kBM) ||
+    if (!make_operand_map(&a, dy, p.type, p.n_out, p.n_rows, p.ld_y, 0, 0, t.cg == 2 ? kBM : kRowBox) ||
         !make_operand_map(&b, w, p.type, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, kBK))
         return "the driver refused an operand's tensor map";
     GroupedArgs k;
@@ -613,13 +668,17 @@ size_t grouped_weight_grad_workspace(const srf_grouped_t& p, int n_sms) {
 namespace {
 
 template <int BN, int CG>
-const char* weight_grad(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& k, uint32_t grid, cudaStream_t stream) {
-    if (grid) {
-        const char* why = launch<kWeightGrad, BN, CG>(a, b, k, grid, stream);
+const char* weight_grad(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& k, const WeightGradPlan& w, cudaStream_t stream) {
+    if (w.grid) {
+        const char* why = launch<kWeightGrad, BN, CG>(a, b, k, w.grid, stream);
         if (why) return why;
     }
-    k_weight_grad_join<BN, CG><<<dim3(k.n_workers - 1 + k.n_groups, join_slices<BN, CG>()), kJoinThreads, 0, stream>>>(k);
-    return nullptr;
+    // Few tiles: all of them, and eight threads to a quad (each tile may have many partial sums); many tiles: the boundaries.
+    const uint64_t tiles = w.across * k.n_groups;
+    constexpr int kFine = join_slices<BN, CG, 8>(), kCoarse = join_slices<BN, CG, 1>();
+    if (tiles * kFine <= 4096) return launch_layer(k_weight_grad_join<BN, CG, 8, true>, 0, kJoinThreads, 1, dim3((uint32_t)tiles, kFine), stream, k);
+    if (tiles <= w.workers) return launch_layer(k_weight_grad_join<BN, CG, 1, true>, 0, kJoinThreads, 1, dim3((uint32_t)tiles, kCoarse), stream, k);
+    return launch_layer(k_weight_grad_join<BN, CG, 1, false>, 0, kJoinThreads, 1, dim3(k.n_workers - 1 + k.n_groups, kCoarse), stream, k);
 }
 
 }  // namespace
@@ -639,11 +698,11 @@ const char* launch_grouped_weight_grad(const srf_grouped_t& p, const uint64_t* o
     if (w.grid && (!make_operand_map(&a, dy, p.type, p.n_out, p.n_rows, p.ld_y, 0, 0, kBK) ||
                    !make_operand_map(&b, x, p.type, p.n_in, p.n_rows, p.ld_x, 0, 0, kBK)))
         return "the driver refused an operand's tensor map";
-    if (w.cg == 2) return weight_grad<256, 2>(a, b, k, w.grid, stream);
+    if (w.cg == 2) return weight_grad<256, 2>(a, b, k, w, stream);
     switch (w.bn) {
-    case 256: return weight_grad<256, 1>(a, b, k, w.grid, stream);
-    case 128: return weight_grad<128, 1>(a, b, k, w.grid, stream);
-    default: return weight_grad<64, 1>(a, b, k, w.grid, stream);
+    case 256: return weight_grad<256, 1>(a, b, k, w, stream);
+    case 128: return weight_grad<128, 1>(a, b, k, w, stream);
+    default: return weight_grad<64, 1>(a, b, k, w, stream);
     }
 }
 

@@ -100,6 +100,8 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     if (CG == 2) cluster_sync(); else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    wait_for_inputs();
+    let_next_start();
 
     bool bad = false, ok = true;
     GroupWalk walk;
@@ -126,13 +128,19 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             Ring<kStages> at_stage;
             uint32_t issued = 0;
             while (ok && next_tile()) {
+                // single CTAs load only the rows that the group has (what lies in the others' place is never stored)
+                const uint32_t boxes = CG == 2 || span.end - m >= (uint32_t)kBM ? kBM / kRowBox : (span.end - m + kRowBox - 1) / kRowBox;
+                const uint32_t bytes = boxes * (kRowBox * kBK) + kBBytes;
                 if (elect_one()) {
                     Ring<kStages> r = at_stage;
                     for (uint32_t k = 0; k < blocks_k; ++k) {
                         if (r.round > 0 && !mbar_wait_one(bar_empty + 8 * r.slot, (r.round - 1) & 1, failed)) { ok = false; break; }
                         const uint32_t bar = lead_full + 8 * r.slot;
-                        pair_expect<CG>(bar, kABytes + kBBytes);
-                        tma_2d<CG>(a0 + r.slot * kABytes, &map_a, bar, (int)(k * kBK), (int)m);
+                        pair_expect<CG>(bar, bytes);
+                        if (CG == 2) tma_2d<CG>(a0 + r.slot * kABytes, &map_a, bar, (int)(k * kBK), (int)m);
+                        else
+                            for (uint32_t i = 0; i < boxes; ++i)
+                                tma_2d<CG>(a0 + r.slot * kABytes + i * (kRowBox * kBK), &map_a, bar, (int)(k * kBK), (int)(m + i * kRowBox));
                         tma_3d<CG>(b0 + r.slot * kBBytes, &map_b, bar, (int)(k * kBK), (int)(tn * BN + rank * kBRows), (int)group);
                         ++issued;
                         r.step();
@@ -292,7 +300,7 @@ const char* launch_grouped_matmul_fp8(const srf_grouped_t& p, const uint64_t* of
     const int sms = sm_count();
     const TileShape t = pick_tile(p, p.n_out, sms, 64);
     CUtensorMap a, b;
-    if (!make_operand_map(&a, x, SRF_TYPE_E4M3, p.n_in, p.n_rows, p.ld_x, 0, 0, kBM) ||
+    if (!make_operand_map(&a, x, SRF_TYPE_E4M3, p.n_in, p.n_rows, p.ld_x, 0, 0, t.cg == 2 ? kBM : kRowBox) ||
         !make_operand_map(&b, w, SRF_TYPE_E4M3, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, t.bn / t.cg))
         return "the driver refused an operand's tensor map";
     Fp8Args k;
@@ -302,11 +310,11 @@ const char* launch_grouped_matmul_fp8(const srf_grouped_t& p, const uint64_t* of
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.out_type == SRF_TYPE_BF16; k.relu = p.activation == SRF_ACT_RELU;
     k.out_row_bytes = p.ld_y * (k.f32 ? 4 : 2); k.error_flags = error_flags;
     const uint32_t grid = tile_grid(p, p.n_out, t, sms);
-    if (t.cg == 2) return launch_tiles(k_grouped_fp8<256, 2>, smem_bytes<256, 2>(), kThreads, 2, grid, stream, a, b, k);
+    if (t.cg == 2) return launch_layer(k_grouped_fp8<256, 2>, smem_bytes<256, 2>(), kThreads, 2, dim3(grid), stream, a, b, k);
     switch (t.bn) {
-    case 256: return launch_tiles(k_grouped_fp8<256, 1>, smem_bytes<256, 1>(), kThreads, 1, grid, stream, a, b, k);
-    case 128: return launch_tiles(k_grouped_fp8<128, 1>, smem_bytes<128, 1>(), kThreads, 1, grid, stream, a, b, k);
-    default: return launch_tiles(k_grouped_fp8<64, 1>, smem_bytes<64, 1>(), kThreads, 1, grid, stream, a, b, k);
+    case 256: return launch_layer(k_grouped_fp8<256, 1>, smem_bytes<256, 1>(), kThreads, 1, dim3(grid), stream, a, b, k);
+    case 128: return launch_layer(k_grouped_fp8<128, 1>, smem_bytes<128, 1>(), kThreads, 1, dim3(grid), stream, a, b, k);
+    default: return launch_layer(k_grouped_fp8<64, 1>, smem_bytes<64, 1>(), kThreads, 1, dim3(grid), stream, a, b, k);
     }
 }
 

@@ -19,9 +19,9 @@ const char* launch_grouped_weight_grad(const srf_grouped_t& p, const uint64_t* o
 const char* launch_grouped_matmul_fp8(const srf_grouped_t& p, const uint64_t* offsets, const void* x, const float* x_scales,
                                       const void* w, const float* w_scales, void* y, unsigned int* error_flags,
                                       cudaStream_t stream);
-void launch_quantize_rows(int type, uint64_t n_rows, const uint64_t* n_rows_used, uint32_t n_cols, const void* in, uint64_t ld_in,
+const char* launch_quantize_rows(int type, uint64_t n_rows, const uint64_t* n_rows_used, uint32_t n_cols, const void* in, uint64_t ld_in,
                           void* out, uint64_t ld_out, float* scales, cudaStream_t stream);
-void launch_quantize_weights(int type, uint32_t n_matrices, uint32_t n_rows, uint32_t n_cols, const void* in, uint64_t ld_in,
+const char* launch_quantize_weights(int type, uint32_t n_matrices, uint32_t n_rows, uint32_t n_cols, const void* in, uint64_t ld_in,
                              uint64_t stride_in, void* out, uint64_t ld_out, uint64_t stride_out, float* scales, cudaStream_t stream);
 
 // Host side of the tensor maps: element size 1 or 2, dims/strides innermost first, 128-byte swizzle, box {128 bytes,
@@ -32,28 +32,35 @@ int sm_count();
 
 // Row tiles of `height` that n_rows samples in n_groups groups can have at most.
 uint64_t max_row_tiles(const srf_grouped_t& p, uint64_t height);
-// Output tiles of a layer or an input gradient with `cols` columns: CG*128 samples x BN columns on CG CTAs.
+// Output tiles of a layer or an input gradient with `cols` columns: CG*128 samples x BN columns on CG CTAs.  A single CTA
+// loads its samples in boxes of kRowBox rows, as many as the tile has.
+constexpr uint32_t kRowBox = 32;
 struct TileShape { int bn, cg; };
 TileShape pick_tile(const srf_grouped_t& p, uint32_t cols, int sms, int smallest);
 // CTAs for them: one per SM, no more than there can be tiles.
 uint32_t tile_grid(const srf_grouped_t& p, uint32_t cols, TileShape t, int sms);
 
-// One persistent launch of a tile kernel; `cg` CTAs to a cluster.
+// One launch of a layer kernel; `cg` CTAs to a cluster.  The kernel may be set up while the one in front of it in the stream
+// still runs (it waits for that one before it touches memory): layers follow one another in chains, and for a few
+// samples the set-up is most of a layer's time.
 template <class Kernel, class... Args>
-const char* launch_tiles(Kernel kernel, int smem, int threads, int cg, uint32_t grid, cudaStream_t stream, const Args&... args) {
-    if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return "cudaFuncSetAttribute failed";
+const char* launch_layer(Kernel kernel, int smem, int threads, int cg, dim3 grid, cudaStream_t stream, const Args&... args) {
+    if (smem > 48 * 1024 && cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return "cudaFuncSetAttribute failed";
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cg;
-    at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cg;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = cg > 1 ? 1 : 0;
+    cfg.numAttrs = cg > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? nullptr : "the layer kernel did not launch";
 }
 

@@ -17,6 +17,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "srf_layers.cuh"
+#include "srf_tile.cuh"
 
 namespace srf {
 
@@ -127,6 +128,8 @@ __global__ void __launch_bounds__(256)
 k_quantize_rows(int bf16, uint64_t n_rows, const uint64_t* __restrict__ n_used, uint32_t n_cols, const uint16_t* __restrict__ in,
                 uint64_t ld_in, unsigned char* __restrict__ out, uint64_t ld_out, float* __restrict__ scales) {
     uint64_t rows = n_rows;
+    tile::wait_for_inputs();
+    tile::let_next_start();
     if (n_used) { const uint64_t u = __ldg((const unsigned long long*)n_used); rows = u < rows ? u : rows; }
     const int lane = threadIdx.x & 31;
     const uint32_t block = blockIdx.y * 2 + (lane >> 4);
@@ -168,6 +171,8 @@ k_quantize_weights(int bf16, uint32_t n_rows, uint32_t n_cols, const uint16_t* _
     const uint32_t bx = blockIdx.x, by = blockIdx.y, mat = blockIdx.z;
     const uint32_t col = bx * 128 + (threadIdx.x & 15) * 8, row0 = by * 128 + (threadIdx.x >> 4);
     const int have = col >= n_cols ? 0 : n_cols - col < 8 ? (int)(n_cols - col) : 8;
+    tile::wait_for_inputs();
+    tile::let_next_start();
     in += mat * stride_in;
     out += mat * stride_out;
     uint4 v[8];
@@ -217,19 +222,19 @@ k_quantize_weights(int bf16, uint32_t n_rows, uint32_t n_cols, const uint16_t* _
 
 }  // namespace
 
-void launch_quantize_rows(int type, uint64_t n_rows, const uint64_t* n_rows_used, uint32_t n_cols, const void* in, uint64_t ld_in,
-                          void* out, uint64_t ld_out, float* scales, cudaStream_t stream) {
-    if (!n_rows) return;
+const char* launch_quantize_rows(int type, uint64_t n_rows, const uint64_t* n_rows_used, uint32_t n_cols, const void* in, uint64_t ld_in,
+                                 void* out, uint64_t ld_out, float* scales, cudaStream_t stream) {
+    if (!n_rows) return nullptr;
     const dim3 grid((uint32_t)((n_rows + 8 * kRowsPerWarp - 1) / (8 * kRowsPerWarp)), (n_cols + 255) / 256);
-    k_quantize_rows<<<grid, 256, 0, stream>>>(type == SRF_TYPE_BF16, n_rows, n_rows_used, n_cols, (const uint16_t*)in, ld_in,
-                                              (unsigned char*)out, ld_out, scales);
+    return launch_layer(k_quantize_rows, 0, 256, 1, grid, stream, (int)(type == SRF_TYPE_BF16), n_rows, n_rows_used, n_cols, (const uint16_t*)in,
+                        ld_in, (unsigned char*)out, ld_out, scales);
 }
 
-void launch_quantize_weights(int type, uint32_t n_matrices, uint32_t n_rows, uint32_t n_cols, const void* in, uint64_t ld_in,
-                             uint64_t stride_in, void* out, uint64_t ld_out, uint64_t stride_out, float* scales, cudaStream_t stream) {
+const char* launch_quantize_weights(int type, uint32_t n_matrices, uint32_t n_rows, uint32_t n_cols, const void* in, uint64_t ld_in,
+                                    uint64_t stride_in, void* out, uint64_t ld_out, uint64_t stride_out, float* scales, cudaStream_t stream) {
     const dim3 grid((n_cols + 127) / 128, (n_rows + 127) / 128, n_matrices);
-    k_quantize_weights<<<grid, 256, 0, stream>>>(type == SRF_TYPE_BF16, n_rows, n_cols, (const uint16_t*)in, ld_in, stride_in,
-                                                 (unsigned char*)out, ld_out, stride_out, scales);
+    return launch_layer(k_quantize_weights, 0, 256, 1, grid, stream, (int)(type == SRF_TYPE_BF16), n_rows, n_cols, (const uint16_t*)in, ld_in,
+                        stride_in, (unsigned char*)out, ld_out, stride_out, scales);
 }
 
 }  // namespace srf

@@ -63,6 +63,11 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
+// Programmatic dependent launch: a kernel's blocks may be set up while the kernel in front of it in the stream still runs.
+// Nothing in global memory is touched in front of wait_for_inputs(), which returns when that kernel has completed.
+__device__ __forceinline__ void wait_for_inputs() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Place in a ring of `N` slots, advanced by all lanes of a warp alike.
 template <int N>
 struct Ring {
