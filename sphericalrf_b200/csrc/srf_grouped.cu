@@ -32,7 +32,8 @@ namespace {
 
 enum Mode { kLayer = 0, kInputGrad = 1, kWeightGrad = 2 };
 
-constexpr int kThreads = 384;                 // TMA, MMA, TMEM owner, spare, two sets of 4 epilogue warps
+constexpr int kThreads = 384;                 // TMA, MMA, TMEM owner, spare, two sets of 4 epilogue warps (four sets: 41.2 us
+                                              // for 1048613 samples 32 -> 64 against 40.4, narrow gradients 46.9 against 44.3)
 constexpr int kBM = 128, kBK = 64;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kABytes = kBM * kBK * 2;
@@ -370,12 +371,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         if (c + 32u * h < cols) {
                             tmem_ld32(d + c + 32 * h, r);
                             tmem_ld_wait(r);
-                            if (p.relu)
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(relu(__uint_as_float(r[i])));
                             uint32_t o[16];
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = pack16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), rs.bf16);
+                            pack32(r, o, rs.bf16, p.relu != 0);
 #pragma unroll
                             for (int u = 0; u < 4; ++u) stage_unit(stage, lane, 4 * h + u, make_uint4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]));
                         }

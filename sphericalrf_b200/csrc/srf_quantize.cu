@@ -140,27 +140,45 @@ k_quantize_rows(int bf16, uint64_t n_rows, const uint64_t* __restrict__ n_used, 
     uint4 v[kRowsPerWarp];
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i) v[i] = row0 + i < rows ? load8(in + (row0 + i) * ld_in + col, have) : make_uint4(0u, 0u, 0u, 0u);
+    // Every lane makes the scale of one of its half's four blocks -- the two divisions of a scale cost as much as all the rest
+    // of a block, and 16 lanes repeating them for every row made the kernel issue-bound (65539 x 2048: 88 us, 82 without).
+    uint32_t mine = 0;
+    bool finite_all = true;
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i) {
         uint32_t top = amax_pattern(v[i], 0u);
 #pragma unroll
         for (int d = 8; d; d >>= 1) top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, d));
         top = max(top & 0xffffu, top >> 16);
-        float f[8];
-        unpack8(v[i], bf16 != 0, f);
-        const bool all_finite = pattern_finite(top, bf16 != 0);
-        float amax = pattern_value(top, bf16 != 0);
-        if (!__all_sync(0xffffffffu, all_finite)) {
+        mine = (lane & (kRowsPerWarp - 1)) == i ? top : mine;
+        finite_all = finite_all && pattern_finite(top, bf16 != 0);
+    }
+    const bool mine_finite = pattern_finite(mine, bf16 != 0);
+    float amax = pattern_value(mine, bf16 != 0);
+    if (!__all_sync(0xffffffffu, finite_all)) {
+#pragma unroll
+        for (int i = 0; i < kRowsPerWarp; ++i) {
+            float f[8];
+            unpack8(v[i], bf16 != 0, f);
             float a = amax_finite(f, 0.f);
 #pragma unroll
             for (int d = 8; d; d >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
-            amax = a;
+            amax = (lane & (kRowsPerWarp - 1)) == i ? a : amax;
         }
-        const BlockScale b = block_scale(amax, all_finite);
-        if (row0 + i < rows) {
-            if (have > 0) store8(out + (row0 + i) * ld_out + col, have, quantize8(f, b));
-            if ((lane & 15) == 0 && block * 128 < n_cols) scales[(uint64_t)block * n_rows + row0 + i] = b.scale;
-        }
+    }
+    const BlockScale own = block_scale(amax, mine_finite);
+    if ((lane & 15) < kRowsPerWarp && row0 + (lane & 15) < rows && block * 128 < n_cols) scales[(uint64_t)block * n_rows + row0 + (lane & 15)] = own.scale;
+    const bool plain_all = __all_sync(0xffffffffu, own.plain);
+#pragma unroll
+    for (int i = 0; i < kRowsPerWarp; ++i) {
+        BlockScale b;
+        b.scale = __shfl_sync(0xffffffffu, own.scale, (lane & 16) | i);
+        b.inverse = __shfl_sync(0xffffffffu, own.inverse, (lane & 16) | i);
+        b.plain = true;
+        if (!plain_all) b.plain = __shfl_sync(0xffffffffu, (int)own.plain, (lane & 16) | i);
+        float f[8];
+        unpack8(v[i], bf16 != 0, f);
+        if (row0 + i < rows && have > 0) store8(out + (row0 + i) * ld_out + col, have, quantize8(f, b));
     }
 }
 

@@ -319,6 +319,23 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// The same with negative values clamped to zero and NaN kept, in one instruction.
+__device__ __forceinline__ uint32_t pack16_relu(float lo, float hi, bool bf16) {
+    uint32_t r;
+    if (bf16) asm("cvt.rn.relu.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.relu.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// 32 sums (as bits) -> 32 values of 16 bits.
+__device__ __forceinline__ void pack32(const uint32_t (&r)[32], uint32_t (&o)[16], bool bf16, bool clamp) {
+    if (clamp) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = pack16_relu(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), bf16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = pack16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), bf16);
+    }
+}
 // NaN stays NaN.
 __device__ __forceinline__ float relu(float v) {
     asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(v));
