@@ -86,18 +86,7 @@ __device__ __forceinline__ BlockScale block_scale(float amax, bool all_finite) {
     return b;
 }
 
-__device__ __forceinline__ uint2 quantize8(const float (&f)[8], const BlockScale& b) {
-    float q[8];
-    if (b.plain) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float q0 = f[i] * b.inverse;
-            q[i] = fmaf(fmaf(-q0, b.scale, f[i]), b.inverse, q0);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = finite(f[i]) ? f[i] / b.scale : __int_as_float(0x7fffffff);
-    }
+__device__ __forceinline__ uint2 to_e4m3(const float (&q)[8]) {
     uint32_t h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -106,6 +95,32 @@ __device__ __forceinline__ uint2 quantize8(const float (&f)[8], const BlockScale
         h[i] = t;
     }
     return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+}
+
+// The short way, two values to an instruction.
+__device__ __forceinline__ uint2 quantize8_plain(const float (&f)[8], float scale, float inverse) {
+    uint64_t down, inv;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(down) : "f"(-scale));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(inv) : "f"(inverse));
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint64_t v, q0, rest;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(f[2 * i]), "f"(f[2 * i + 1]));
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q0) : "l"(v), "l"(inv));
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(rest) : "l"(q0), "l"(down), "l"(v));
+        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(q0) : "l"(rest), "l"(inv));
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(q[2 * i]), "=f"(q[2 * i + 1]) : "l"(q0));
+    }
+    return to_e4m3(q);
+}
+
+__device__ __forceinline__ uint2 quantize8(const float (&f)[8], const BlockScale& b) {
+    if (b.plain) return quantize8_plain(f, b.scale, b.inverse);
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = finite(f[i]) ? f[i] / b.scale : __int_as_float(0x7fffffff);
+    return to_e4m3(q);
 }
 
 __device__ __forceinline__ float pattern_value(uint32_t h, bool bf16) {
@@ -138,10 +153,18 @@ k_quantize_rows(int bf16, uint64_t n_rows, const uint64_t* __restrict__ n_used, 
     const uint32_t col = block * 128 + (lane & 15) * 8;
     const int have = col >= n_cols ? 0 : n_cols - col < 8 ? (int)(n_cols - col) : 8;
     uint4 v[kRowsPerWarp];
+    const bool full = (blockIdx.y + 1) * 256 <= n_cols && row0 + kRowsPerWarp <= rows;       // no edge: the same for the warp
+    in += row0 * ld_in;
+    out += row0 * ld_out;
+    if (full) {
 #pragma unroll
-    for (int i = 0; i < kRowsPerWarp; ++i) v[i] = row0 + i < rows ? load8(in + (row0 + i) * ld_in + col, have) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < kRowsPerWarp; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(in + i * ld_in + col));
+    } else {
+#pragma unroll
+        for (int i = 0; i < kRowsPerWarp; ++i) v[i] = row0 + i < rows ? load8(in + i * ld_in + col, have) : make_uint4(0u, 0u, 0u, 0u);
+    }
     // Every lane makes the scale of one of its half's four blocks -- the two divisions of a scale cost as much as all the rest
-    // of a block, and 16 lanes repeating them for every row made the kernel issue-bound (65539 x 2048: 88 us, 82 without).
+    // of a block, and 16 lanes repeating them for every row made the kernel issue-bound (65539 x 2048: 88 us, 82 without it).
     uint32_t mine = 0;
     bool finite_all = true;
 #pragma unroll
@@ -169,6 +192,16 @@ k_quantize_rows(int bf16, uint64_t n_rows, const uint64_t* __restrict__ n_used, 
     const BlockScale own = block_scale(amax, mine_finite);
     if ((lane & 15) < kRowsPerWarp && row0 + (lane & 15) < rows && block * 128 < n_cols) scales[(uint64_t)block * n_rows + row0 + (lane & 15)] = own.scale;
     const bool plain_all = __all_sync(0xffffffffu, own.plain);
+    if (full && plain_all) {
+#pragma unroll
+        for (int i = 0; i < kRowsPerWarp; ++i) {
+            float f[8];
+            unpack8(v[i], bf16 != 0, f);
+            *reinterpret_cast<uint2*>(out + i * ld_out + col) = quantize8_plain(f, __shfl_sync(0xffffffffu, own.scale, (lane & 16) | i),
+                                                                                __shfl_sync(0xffffffffu, own.inverse, (lane & 16) | i));
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i) {
         BlockScale b;
@@ -178,7 +211,7 @@ k_quantize_rows(int bf16, uint64_t n_rows, const uint64_t* __restrict__ n_used, 
         if (!plain_all) b.plain = __shfl_sync(0xffffffffu, (int)own.plain, (lane & 16) | i);
         float f[8];
         unpack8(v[i], bf16 != 0, f);
-        if (row0 + i < rows && have > 0) store8(out + (row0 + i) * ld_out + col, have, quantize8(f, b));
+        if (row0 + i < rows && have > 0) store8(out + i * ld_out + col, have, quantize8(f, b));
     }
 }
 

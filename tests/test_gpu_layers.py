@@ -344,7 +344,7 @@ def values(rows, cols, dtype, seed, lead=()):
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
-@pytest.mark.parametrize("rows,cols,used", [(1, 1, None), (1, 128, None), (37, 129, None), (70, 100, 33), (9, 1000, 9), (130, 2048, 0), (40, 256, 99)])
+@pytest.mark.parametrize("rows,cols,used", [(1, 1, None), (1, 128, None), (37, 129, None), (70, 100, 33), (9, 1000, 9), (130, 2048, 0), (40, 256, 99), (133, 512, None)])
 def test_quantize_rows(r, rows, cols, used, kind):
     type_id, dt = TYPES[kind]
     v = values(rows, cols, dt, rows + cols)
