@@ -153,6 +153,8 @@ SHAPES = [
     ([260, 900, 64, 2500], 512, 768, 0, 0),
     ([20000, 3, 0, 18001], 136, 600, 2, 9),
     ([9000, 30000], 700, 264, 0, 0),
+    ([700, 90, 0, 1500, 64, 333, 1, 2000], 1100, 600, 0, 11),
+    ([30] * 160 + [0] * 3 + [500, 7], 40, 72, 5, 0),
 ]
 
 
@@ -267,13 +269,14 @@ def test_bad_offsets_are_reported(r, offsets):
     assert bool((dw[0] == POISON).all()) and bool((dw[4] == POISON).all())
 
 
-def test_weight_grad_is_the_same_every_time(r):
-    c = Case([5000, 0, 321, 70000], 72, 200, "bf16", 11)
-    p = c.layer(abi.TYPE_F32, ld_w=72, group_stride=0)
+@pytest.mark.parametrize("sizes,n_in,n_out", [([5000, 0, 321, 70000], 72, 200), ([3000, 900, 0, 2500, 4000], 1024, 1032)])
+def test_weight_grad_is_the_same_every_time(r, sizes, n_in, n_out):
+    c = Case(sizes, n_in, n_out, "bf16", 11)
+    p = c.layer(abi.TYPE_F32, ld_w=n_in, group_stride=0)
     got = []
     for k in range(3):
         space = torch.full((r.grouped_weight_grad_workspace(p),), 255 - k, dtype=torch.uint8, device="cuda")
-        dw = torch.full((4, 200, 72), POISON, device="cuda")
+        dw = torch.full((len(sizes), n_out, n_in), POISON, device="cuda")
         r.grouped_weight_grad_device(p, c.offsets, c.dy, c.x, dw, space)
         torch.cuda.synchronize()
         got.append(dw)
