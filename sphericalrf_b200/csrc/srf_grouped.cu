@@ -531,10 +531,10 @@ WeightGradPlan plan_weight_grad(const srf_grouped_t& p, int sms) {
     const uint64_t units = max_row_tiles(p, kBK) * w.across, teams = sms / w.cg;
     const uint64_t busy = units < teams ? units : teams;
     // All teams together walk the samples once per tile of a group that a team works on; samples beyond what L2 holds are
-    // taken part by part.
+    // taken in two parts (16389 x 2048 x 2048 with its input gradient: 355 us in one, 305 in two, 310 in three, 329 in
+    // four -- every part cuts as many tiles again).
     const uint64_t bytes = p.n_rows * (p.n_in + p.n_out) * 2;
-    uint64_t parts = w.across < 8 ? 1 : bytes / (64ull << 20) + 1;
-    if (parts > 4) parts = 4;
+    const uint64_t parts = w.across >= 8 && bytes > (64ull << 20) ? 2 : 1;
     w.grid = (uint32_t)busy * w.cg;
     w.workers = (uint32_t)(busy * parts);
     if (!w.workers) w.workers = 1;

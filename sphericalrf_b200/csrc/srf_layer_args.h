@@ -77,7 +77,7 @@ inline std::string refuse_grouped(const srf_grouped_t* in, LayerCall call, srf_g
     if (!p->ld_w) p->ld_w = p->n_in;
     if (!p->ld_y) p->ld_y = p->n_out;
     if (p->ld_x >= (1ull << 36) || p->ld_w >= (1ull << 36) || p->ld_y >= (1ull << 36)) return "row strides must be less than 2^36";
-    if (!p->group_stride) p->group_stride = p->n_out * p->ld_w;
+    if (!p->group_stride || p->n_groups == 1) p->group_stride = p->n_out * p->ld_w;
     return "";
 }
 
