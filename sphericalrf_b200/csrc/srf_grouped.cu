@@ -16,6 +16,11 @@
 // Large layers run on pairs of CTAs (CG = 2): one instruction computes 256 x 256 outputs on two SMs, each of which
 // loads its own 128 rows of A and half of B, so that an operand byte from L2 serves twice as many products.
 //
+// The tensor core's additions to an accumulator truncate, so that a long sum's error grows with its length (2-norm 2.1e-6 at
+// 2048 products, 9e-6 at 8192, where fp32 additions one by one have 4e-7): nothing beside a rounding to 16 bits, but not
+// what a result in fp32 should have.  LONG kernels therefore start a new accumulator every 512 products and add those in
+// registers, rounded (5e-7 at any length); both sets of epilogue warps work on every tile then, half of its columns each.
+//
 // A tile's rows behind its group's end hold the next group's samples: harmless in the first two products (an output row
 // depends on its own sample alone and those rows are not stored).  In the weight gradient they would be summed, so the
 // rows of the last stage of a group are zeroed in shared memory, in both operands (a NaN of the next group must not
@@ -35,6 +40,7 @@ enum Mode { kLayer = 0, kInputGrad = 1, kWeightGrad = 2 };
 constexpr int kThreads = 384;                 // TMA, MMA, TMEM owner, spare, two sets of 4 epilogue warps (four sets: 41.2 us
                                               // for 1048613 samples 32 -> 64 against 40.4, narrow gradients 46.9 against 44.3)
 constexpr int kBM = 128, kBK = 64;
+constexpr uint32_t kChunk = 8;                // stages to an accumulator in LONG kernels
 constexpr uint32_t kTmemCols = 512;
 constexpr int kABytes = kBM * kBK * 2;
 constexpr int kStoreBytes = 8 * 4096;         // staging of the epilogue warps
@@ -171,7 +177,7 @@ __device__ __forceinline__ void zero_rows(unsigned char* stage, int blocks, int 
     }
 }
 
-template <int MODE, int BN, int CG>
+template <int MODE, int BN, int CG, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1)
 k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GroupedArgs p) {
     constexpr int kStages = n_stages<BN, CG>(), kAccs = n_accs<BN>();
@@ -197,7 +203,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     // `acc_full` are signalled in both CTAs.
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) { mbar_init(bar_full + 8 * i, CG); mbar_init(bar_empty + 8 * i, 1); }
-        for (int i = 0; i < kAccs; ++i) { mbar_init(bar_acc_full + 8 * i, 1); mbar_init(bar_acc_empty + 8 * i, 4 * CG); }
+        for (int i = 0; i < kAccs; ++i) { mbar_init(bar_acc_full + 8 * i, 1); mbar_init(bar_acc_empty + 8 * i, (LONG ? 8 : 4) * CG); }
         mbar_init(bar_tail, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *failed = 0;
@@ -214,139 +220,235 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 
     bool bad = false, ok = true;
     Pieces<MODE, CG> pieces;
-    const bool storing = MODE != kWeightGrad && warp >= 4;       // the two sets of epilogue warps take every other piece
+    const bool storing = !LONG && warp >= 4;       // the two sets of epilogue warps take every other piece
     pieces.init(p, MODE == kWeightGrad ? all_units<MODE, CG>(p, tiles_m * tiles_n, &bad) : 0, storing ? (warp - 4) >> 2 : 0, storing ? 2 : 1);
     Piece t;
 
-    if (warp == 0) {
-        // ---- operand loads: one thread, but for the zeroing of a group's last stage ----
-        const uint32_t lead_full = CG == 2 ? leader_addr(bar_full) : bar_full;
-        const uint32_t a0 = smem_u32(sm_a), b0 = smem_u32(sm_b);
-        Ring<kStages> at;
-        uint32_t issued = 0, tails = 0;
-        while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
-            const int am = (int)(t.m + rank * kBM), bn = (int)(t.n * BN + rank * kBRows);
-            // weight gradient: the group's last stage, if it is of this piece and not a full one
-            const uint32_t deep = t.span.end - t.span.begin;
-            const bool tail = MODE == kWeightGrad && (t.k0 + t.k_stages) * kBK > deep;
-            // single CTAs load only the rows that the group has (what lies in the others' place is never stored)
-            const uint32_t boxes = MODE == kWeightGrad || CG == 2 || t.span.end - t.m >= (uint32_t)kBM ? kBM / kRowBox : (t.span.end - t.m + kRowBox - 1) / kRowBox;
-            const uint32_t bytes = boxes * (kABytes / (kBM / kRowBox)) + kBBytes;
-            if (elect_one()) {
-                Ring<kStages> r = at;
-                for (uint32_t k = 0; k < t.k_stages; ++k) {
-                    if (r.round > 0 && !mbar_wait_one(bar_empty + 8 * r.slot, (r.round - 1) & 1, failed)) { ok = false; break; }
-                    const bool last = tail && k + 1 == t.k_stages;
-                    const uint32_t a = a0 + r.slot * kABytes, b = b0 + r.slot * kBBytes, bar = last ? bar_tail : lead_full + 8 * r.slot;
-                    if (last) mbar_expect(bar_tail, bytes);
-                    else pair_expect<CG>(bar, bytes);
-                    const int kk = (int)((t.k0 + k) * kBK);
-                    if (kAColumns) {
+    if (warp < 4) {
+        if (LONG && BN == 256) regs_for_issue();
+        if (warp == 0) {
+            // ---- operand loads: one thread, but for the zeroing of a group's last stage ----
+            const uint32_t lead_full = CG == 2 ? leader_addr(bar_full) : bar_full;
+            const uint32_t a0 = smem_u32(sm_a), b0 = smem_u32(sm_b);
+            Ring<kStages> at;
+            uint32_t issued = 0, tails = 0;
+            while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
+                const int am = (int)(t.m + rank * kBM), bn = (int)(t.n * BN + rank * kBRows);
+                // weight gradient: the group's last stage, if it is of this piece and not a full one
+                const uint32_t deep = t.span.end - t.span.begin;
+                const bool tail = MODE == kWeightGrad && (t.k0 + t.k_stages) * kBK > deep;
+                // single CTAs load only the rows that the group has (what lies in the others' place is never stored)
+                const uint32_t boxes = MODE == kWeightGrad || CG == 2 || t.span.end - t.m >= (uint32_t)kBM ? kBM / kRowBox : (t.span.end - t.m + kRowBox - 1) / kRowBox;
+                const uint32_t bytes = boxes * (kABytes / (kBM / kRowBox)) + kBBytes;
+                if (elect_one()) {
+                    Ring<kStages> r = at;
+                    for (uint32_t k = 0; k < t.k_stages; ++k) {
+                        if (r.round > 0 && !mbar_wait_one(bar_empty + 8 * r.slot, (r.round - 1) & 1, failed)) { ok = false; break; }
+                        const bool last = tail && k + 1 == t.k_stages;
+                        const uint32_t a = a0 + r.slot * kABytes, b = b0 + r.slot * kBBytes, bar = last ? bar_tail : lead_full + 8 * r.slot;
+                        if (last) mbar_expect(bar_tail, bytes);
+                        else pair_expect<CG>(bar, bytes);
+                        const int kk = (int)((t.k0 + k) * kBK);
+                        if (kAColumns) {
 #pragma unroll
-                        for (int i = 0; i < kBM / 64; ++i) tma_2d<CG>(a + i * 8192, &map_a, bar, am + 64 * i, (int)t.span.begin + kk);
-                    } else if (CG == 2) {
-                        tma_2d<CG>(a, &map_a, bar, kk, am);
-                    } else {
-                        for (uint32_t i = 0; i < boxes; ++i) tma_2d<CG>(a + i * (kRowBox * 128), &map_a, bar, kk, am + (int)(i * kRowBox));
+                            for (int i = 0; i < kBM / 64; ++i) tma_2d<CG>(a + i * 8192, &map_a, bar, am + 64 * i, (int)t.span.begin + kk);
+                        } else if (CG == 2) {
+                            tma_2d<CG>(a, &map_a, bar, kk, am);
+                        } else {
+                            for (uint32_t i = 0; i < boxes; ++i) tma_2d<CG>(a + i * (kRowBox * 128), &map_a, bar, kk, am + (int)(i * kRowBox));
+                        }
+                        if (MODE == kLayer) {
+                            tma_3d<CG>(b, &map_b, bar, kk, bn, (int)t.group);
+                        } else if (MODE == kInputGrad) {
+#pragma unroll
+                            for (int i = 0; i < kBRows / 64; ++i) tma_3d<CG>(b + i * 8192, &map_b, bar, bn + 64 * i, kk, (int)t.group);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < kBRows / 64; ++i) tma_2d<CG>(b + i * 8192, &map_b, bar, bn + 64 * i, (int)t.span.begin + kk);
+                        }
+                        ++issued;
+                        r.step();
                     }
-                    if (MODE == kLayer) {
-                        tma_3d<CG>(b, &map_b, bar, kk, bn, (int)t.group);
-                    } else if (MODE == kInputGrad) {
-#pragma unroll
-                        for (int i = 0; i < kBRows / 64; ++i) tma_3d<CG>(b + i * 8192, &map_b, bar, bn + 64 * i, kk, (int)t.group);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < kBRows / 64; ++i) tma_2d<CG>(b + i * 8192, &map_b, bar, bn + 64 * i, (int)t.span.begin + kk);
-                    }
-                    ++issued;
-                    r.step();
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                at.skip(t.k_stages);
+                if (tail) {
+                    // When the last stage has landed, zero the next group's samples up to the next 16 (an instruction's
+                    // depth), then report the stage.
+                    const uint32_t q = at.slot ? at.slot - 1 : kStages - 1;
+                    ok = mbar_wait(bar_tail, tails++ & 1, failed);
+                    const int r0 = (int)(deep - (t.k0 + t.k_stages - 1) * kBK), r1 = (r0 + 15) & ~15;
+                    zero_rows(sm_a + q * kABytes, kBM / 64, r0, r1);
+                    zero_rows(sm_b + q * kBBytes, kBRows / 64, r0, r1);
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && ok) pair_arrive<CG>(lead_full + 8 * q);
+                    __syncwarp();
                 }
             }
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            at.skip(t.k_stages);
-            if (tail) {
-                // When the last stage has landed, zero the next group's samples up to the next 16 (an instruction's
-                // depth), then report the stage.
-                const uint32_t q = at.slot ? at.slot - 1 : kStages - 1;
-                ok = mbar_wait(bar_tail, tails++ & 1, failed);
-                const int r0 = (int)(deep - (t.k0 + t.k_stages - 1) * kBK), r1 = (r0 + 15) & ~15;
-                zero_rows(sm_a + q * kABytes, kBM / 64, r0, r1);
-                zero_rows(sm_b + q * kBBytes, kBRows / 64, r0, r1);
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0 && ok) pair_arrive<CG>(lead_full + 8 * q);
-                __syncwarp();
+            // Copies may still be on their way when another warp gave up: they must land before the CTA (or pair) leaves.
+            if ((!ok || *failed) && rank == 0) drain_ring<kStages>(bar_full, issued);
+        } else if (warp == 1 && rank == 0) {
+            // ---- matrix instructions: one thread ----
+            const uint32_t idesc = idesc_shape(CG * kBM, BN) | (p.bf16 ? (1u << 7) | (1u << 10) : 0u) | (kAColumns ? 1u << 15 : 0u) | (kBColumns ? 1u << 16 : 0u);
+            const uint64_t desc_a = operand_desc(smem_u32(sm_a), kAColumns ? 8192 : 16, 1024), desc_b = operand_desc(smem_u32(sm_b), kBColumns ? 8192 : 16, 1024);
+            constexpr uint32_t kStepA = kAColumns ? 2048 : 32, kStepB = kBColumns ? 2048 : 32;      // bytes of 16 summed indices
+            Ring<kStages> at;
+            Ring<kAccs> acc;
+            while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
+                if (elect_one()) {
+                    Ring<kStages> r = at;
+                    Ring<kAccs> to = acc;
+                    const uint32_t deep = t.span.end - t.span.begin;
+                    for (uint32_t k0 = 0; ok && k0 < t.k_stages; k0 += LONG ? kChunk : t.k_stages) {
+                        // one accumulator
+                        const uint32_t k1 = LONG && t.k_stages - k0 > kChunk ? k0 + kChunk : t.k_stages;
+                        if (to.round > 0 && !mbar_wait_one(bar_acc_empty + 8 * to.slot, (to.round - 1) & 1, failed)) { ok = false; break; }
+                        const uint32_t d = tmem + to.slot * BN;
+                        for (uint32_t k = k0; k < k1; ++k) {
+                            if (!mbar_wait_one(bar_full + 8 * r.slot, r.round & 1, failed)) { ok = false; break; }
+                            tc_fence_after();
+                            const uint64_t da = desc_at(desc_a, r.slot * kABytes), db = desc_at(desc_b, r.slot * kBBytes);
+                            const uint32_t rows = deep - (t.k0 + k) * kBK;
+                            if (MODE == kWeightGrad && rows < (uint32_t)kBK) {
+                                pair_acquire<CG>();                // the other CTA zeroed rows of its operands
+                                for (uint32_t q = 0; q < (rows + 15) / 16; ++q) mma_f16<CG>(d, desc_at(da, q * kStepA), desc_at(db, q * kStepB), idesc, ((k - k0) | q) != 0);
+                            } else {
+#pragma unroll
+                                for (uint32_t q = 0; q < kBK / 16; ++q) mma_f16<CG>(d, desc_at(da, q * kStepA), desc_at(db, q * kStepB), idesc, ((k - k0) | q) != 0);
+                            }
+                            mma_commit<CG>(bar_empty + 8 * r.slot);
+                            r.step();
+                        }
+                        if (ok) mma_commit<CG>(bar_acc_full + 8 * to.slot);
+                        to.step();
+                    }
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                at.skip(t.k_stages);
+                acc.skip(LONG ? (t.k_stages + kChunk - 1) / kChunk : 1);
             }
         }
-        // Copies may still be on their way when another warp gave up: they must land before the CTA (or pair) leaves.
-        if ((!ok || *failed) && rank == 0) drain_ring<kStages>(bar_full, issued);
-    } else if (warp == 1 && rank == 0) {
-        // ---- matrix instructions: one thread ----
-        const uint32_t idesc = idesc_shape(CG * kBM, BN) | (p.bf16 ? (1u << 7) | (1u << 10) : 0u) | (kAColumns ? 1u << 15 : 0u) | (kBColumns ? 1u << 16 : 0u);
-        const uint64_t desc_a = operand_desc(smem_u32(sm_a), kAColumns ? 8192 : 16, 1024), desc_b = operand_desc(smem_u32(sm_b), kBColumns ? 8192 : 16, 1024);
-        constexpr uint32_t kStepA = kAColumns ? 2048 : 32, kStepB = kBColumns ? 2048 : 32;      // bytes of 16 summed indices
-        Ring<kStages> at;
+    } else if (LONG) {
+        // ---- accumulators to sums, finished sums to memory ----
+        if (BN == 256) regs_for_sums();
+        constexpr int kCols = BN / 2;                 // columns of one set
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        unsigned char* stage = sm_store + (warp - 4) * 4096;
+        const uint32_t lead_acc_empty = CG == 2 ? leader_addr(bar_acc_empty) : bar_acc_empty;
         Ring<kAccs> acc;
         while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
-            if (elect_one()) {
-                Ring<kStages> r = at;
-                const uint32_t d = tmem + acc.slot * BN, deep = t.span.end - t.span.begin;
-                if (acc.round > 0) ok = mbar_wait_one(bar_acc_empty + 8 * acc.slot, (acc.round - 1) & 1, failed);
-                for (uint32_t k = 0; ok && k < t.k_stages; ++k) {
-                    if (!mbar_wait_one(bar_full + 8 * r.slot, r.round & 1, failed)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint64_t da = desc_at(desc_a, r.slot * kABytes), db = desc_at(desc_b, r.slot * kBBytes);
-                    const uint32_t rows = deep - (t.k0 + k) * kBK;
-                    if (MODE == kWeightGrad && rows < (uint32_t)kBK) {
-                        pair_acquire<CG>();                // the other CTA zeroed rows of its operands
-                        for (uint32_t q = 0; q < (rows + 15) / 16; ++q) mma_f16<CG>(d, desc_at(da, q * kStepA), desc_at(db, q * kStepB), idesc, (k | q) != 0);
-                    } else {
+            uint64_t sum[kCols / 2];
 #pragma unroll
-                        for (uint32_t q = 0; q < kBK / 16; ++q) mma_f16<CG>(d, desc_at(da, q * kStepA), desc_at(db, q * kStepB), idesc, (k | q) != 0);
+            for (int i = 0; i < kCols / 2; ++i) sum[i] = 0ull;
+            for (uint32_t k = 0; k < t.k_stages; k += kChunk) {
+                if (!mbar_wait(bar_acc_full + 8 * acc.slot, acc.round & 1, failed)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t d = tmem + acc.slot * BN + half * kCols + ((uint32_t)(quarter * 32) << 16);
+                uint32_t r[2][32];
+                tmem_ld32(d, r[0]);
+#pragma unroll
+                for (int c = 0; c < kCols / 32; ++c) {
+                    tmem_ld_wait(r[c & 1]);
+                    if (c + 1 < kCols / 32) {
+                        tmem_ld32(d + 32 * (c + 1), r[(c + 1) & 1]);
+                    } else {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) pair_arrive_read<CG>(lead_acc_empty + 8 * acc.slot);
                     }
-                    mma_commit<CG>(bar_empty + 8 * r.slot);
-                    r.step();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) add2(sum[16 * c + i], pair_of(r[c & 1][2 * i], r[c & 1][2 * i + 1]));
                 }
-                if (ok) mma_commit<CG>(bar_acc_full + 8 * acc.slot);
+                acc.step();
             }
-            ok = __all_sync(0xffffffffu, ok);
-            at.skip(t.k_stages);
-            acc.step();
+            if (!ok) break;
+            const bool partial = MODE == kWeightGrad && !t.whole;
+            const uint32_t row0 = t.m + rank * kBM + quarter * 32, end = MODE == kWeightGrad ? p.out_rows : t.span.end;
+            const uint32_t col0 = t.n * BN + half * kCols;
+            RowStore rs;
+            rs.bf16 = p.bf16 != 0;
+            rs.f32 = partial || p.f32;
+            rs.gate = nullptr;
+            rs.gate_row_bytes = p.gate_row_bytes;
+            rs.rows = row0 >= end ? 0u : end - row0 < 32 ? end - row0 : 32u;
+            unsigned char* out;
+            if (partial) {
+                // slot 0: the tile began with an earlier worker; slot 1: it goes on with the next one
+                out = reinterpret_cast<unsigned char*>(p.partial + (((size_t)t.worker * 2 + (t.first ? 1 : 0)) * CG + rank) * kBM * BN) +
+                      ((size_t)quarter * 32 * BN + half * kCols) * 4;
+                rs.row_bytes = BN * 4;
+            } else {
+                out = p.out + (MODE == kWeightGrad ? t.group * p.out_group_bytes : 0ull) + row0 * p.out_row_bytes + (size_t)col0 * (rs.f32 ? 4 : 2);
+                rs.row_bytes = p.out_row_bytes;
+            }
+            const uint32_t cols = col0 >= p.out_cols ? 0u : p.out_cols - col0 < (uint32_t)kCols ? p.out_cols - col0 : (uint32_t)kCols;
+            if (rs.f32) {
+#pragma unroll
+                for (int c = 0; c < kCols; c += 32) {
+                    if ((uint32_t)c >= cols) continue;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        float v[4] = {lo_of(sum[c / 2 + 2 * u]), hi_of(sum[c / 2 + 2 * u]), lo_of(sum[c / 2 + 2 * u + 1]), hi_of(sum[c / 2 + 2 * u + 1])};
+                        if (MODE == kLayer && p.relu) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[e] = relu(v[e]);
+                        }
+                        stage_unit(stage, lane, u, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+                    }
+                    rs.bytes = (cols - c < 32u ? cols - c : 32u) * 4u;
+                    rs.out = out + (size_t)c * 4;
+                    if (MODE == kInputGrad && p.gate) {
+                        uint4 hv[8];
+                        rs.gate = p.gate + row0 * p.gate_row_bytes + (size_t)(col0 + c) * 2;
+                        load_gate(rs, hv);
+                        store_rows<true>(rs, stage, hv);
+                    } else {
+                        store_rows(rs, stage);
+                    }
+                }
+            } else if (MODE == kWeightGrad) {
+                constexpr int kPer = kCols < 64 ? kCols : 64;
+#pragma unroll
+                for (int c = 0; c < kCols; c += kPer) {
+                    if ((uint32_t)c >= cols) continue;
+#pragma unroll
+                    for (int u = 0; u < kPer / 8; ++u) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = pack16(lo_of(sum[c / 2 + 4 * u + e]), hi_of(sum[c / 2 + 4 * u + e]), rs.bf16);
+                        stage_unit(stage, lane, u, make_uint4(w[0], w[1], w[2], w[3]));
+                    }
+                    rs.bytes = (cols - c < (uint32_t)kPer ? cols - c : (uint32_t)kPer) * 2u;
+                    rs.out = out + (size_t)c * 2;
+                    store_rows(rs, stage);
+                }
+            }
         }
-    } else if (warp >= 4) {
+    } else {
         // ---- finished accumulators to memory ----
         const int quarter = warp & 3, set = (warp - 4) >> 2;
         unsigned char* stage = sm_store + (warp - 4) * 4096;
         const uint32_t lead_acc_empty = CG == 2 ? leader_addr(bar_acc_empty) : bar_acc_empty;
         uint32_t acc = set, acc_round = 0;
-        if (MODE == kWeightGrad && set) pieces.next(p, tiles_m, tiles_n, &t, &bad);
         while (pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
             RowStore rs;
             rs.bf16 = p.bf16 != 0;
             rs.gate = nullptr;
             rs.gate_row_bytes = p.gate_row_bytes;
-            const bool partial = MODE == kWeightGrad && !t.whole;
             const bool gated = MODE == kInputGrad && p.gate;
-            rs.f32 = partial || p.f32;
+            rs.f32 = p.f32;
             const uint32_t row0 = t.m + rank * kBM + quarter * 32;
-            const uint32_t end = MODE == kWeightGrad ? p.out_rows : t.span.end;
-            rs.rows = row0 >= end ? 0u : end - row0 < 32 ? end - row0 : 32u;
+            rs.rows = row0 >= t.span.end ? 0u : t.span.end - row0 < 32 ? t.span.end - row0 : 32u;
             const uint32_t col0 = t.n * BN;
             const uint32_t cols = p.out_cols - col0 < (uint32_t)BN ? p.out_cols - col0 : (uint32_t)BN;
-            unsigned char* out;
-            if (partial) {
-                // slot 0: the tile began with an earlier worker; slot 1: it goes on with the next one
-                out = reinterpret_cast<unsigned char*>(p.partial + (((size_t)t.worker * 2 + (t.first ? 1 : 0)) * CG + rank) * kBM * BN) + (size_t)quarter * 32 * BN * 4;
-                rs.row_bytes = BN * 4;
-            } else {
-                out = p.out + (MODE == kWeightGrad ? t.group * p.out_group_bytes : 0ull) + row0 * p.out_row_bytes;
-                rs.row_bytes = p.out_row_bytes;
-            }
+            unsigned char* out = p.out + row0 * p.out_row_bytes;
+            rs.row_bytes = p.out_row_bytes;
             const uint32_t per = rs.f32 ? 32u : 64u, size = rs.f32 ? 4u : 2u;
             auto piece = [&](uint32_t c) {
                 rs.bytes = (cols - c < per ? cols - c : per) * size;
-                rs.out = out + (size_t)(partial ? c : col0 + c) * size;
+                rs.out = out + (size_t)(col0 + c) * size;
                 if (gated) rs.gate = p.gate + row0 * p.gate_row_bytes + (size_t)(col0 + c) * 2;
             };
             uint4 hv[8];
@@ -396,7 +498,6 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             }
             acc += 2;
             if (acc >= kAccs) { acc -= kAccs; ++acc_round; }
-            if (MODE == kWeightGrad && !pieces.next(p, tiles_m, tiles_n, &t, &bad)) break;     // the other set's piece
         }
     }
     if ((bad || (!ok && lane == 0)) && p.error_flags) atomicOr(p.error_flags, (ok ? 0u : 2u) | (bad ? 16u : 0u));
@@ -541,10 +642,20 @@ WeightGradPlan plan_weight_grad(const srf_grouped_t& p, int sms) {
     return w;
 }
 
-template <int MODE, int BN, int CG>
+template <int MODE, int BN, int CG, bool LONG>
 const char* launch(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& args, uint32_t grid, cudaStream_t stream) {
     static_assert(smem_bytes<BN, CG>() <= 227 * 1024, "shared memory of one SM");
-    return launch_layer(k_grouped<MODE, BN, CG>, smem_bytes<BN, CG>(), kThreads, CG, dim3(grid), stream, a, b, args);
+    return launch_layer(k_grouped<MODE, BN, CG, LONG>, smem_bytes<BN, CG>(), kThreads, CG, dim3(grid), stream, a, b, args);
+}
+
+template <int MODE>
+const char* launch_long(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& k, TileShape t, uint32_t grid, cudaStream_t stream) {
+    if (t.cg == 2) return launch<MODE, 256, 2, true>(a, b, k, grid, stream);
+    switch (t.bn) {
+    case 256: return launch<MODE, 256, 1, true>(a, b, k, grid, stream);
+    case 128: return launch<MODE, 128, 1, true>(a, b, k, grid, stream);
+    default: return launch<MODE, 64, 1, true>(a, b, k, grid, stream);
+    }
 }
 
 }  // namespace
@@ -613,7 +724,7 @@ const char* launch_grouped_matmul(const srf_grouped_t& p, const uint64_t* offset
                                   unsigned int* error_flags, cudaStream_t stream) {
     if (!p.n_rows) return nullptr;
     const int sms = sm_count();
-    const TileShape t = pick_tile(p, p.n_out, sms, 32);
+    const TileShape t = pick_tile(p, p.n_out, sms, p.out_type == SRF_TYPE_F32 && p.n_in > kChunk * kBK ? 64 : 32);
     CUtensorMap a, b;
     if (!make_operand_map(&a, x, p.type, p.n_in, p.n_rows, p.ld_x, 0, 0, t.cg == 2 ? kBM : kRowBox) ||
         !make_operand_map(&b, w, p.type, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, t.bn / t.cg))
@@ -624,12 +735,13 @@ const char* launch_grouped_matmul(const srf_grouped_t& p, const uint64_t* offset
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16; k.relu = p.activation == SRF_ACT_RELU;
     k.out_row_bytes = p.ld_y * (k.f32 ? 4 : 2); k.out_cols = p.n_out; k.depth = p.n_in; k.error_flags = error_flags;
     const uint32_t grid = tile_grid(p, p.n_out, t, sms);
-    if (t.cg == 2) return launch<kLayer, 256, 2>(a, b, k, grid, stream);
+    if (k.f32 && p.n_in > kChunk * kBK) return launch_long<kLayer>(a, b, k, t, grid, stream);
+    if (t.cg == 2) return launch<kLayer, 256, 2, false>(a, b, k, grid, stream);
     switch (t.bn) {
-    case 256: return launch<kLayer, 256, 1>(a, b, k, grid, stream);
-    case 128: return launch<kLayer, 128, 1>(a, b, k, grid, stream);
-    case 64: return launch<kLayer, 64, 1>(a, b, k, grid, stream);
-    default: return launch<kLayer, 32, 1>(a, b, k, grid, stream);
+    case 256: return launch<kLayer, 256, 1, false>(a, b, k, grid, stream);
+    case 128: return launch<kLayer, 128, 1, false>(a, b, k, grid, stream);
+    case 64: return launch<kLayer, 64, 1, false>(a, b, k, grid, stream);
+    default: return launch<kLayer, 32, 1, false>(a, b, k, grid, stream);
     }
 }
 
@@ -649,11 +761,12 @@ const char* launch_grouped_input_grad(const srf_grouped_t& p, const uint64_t* of
     k.out_row_bytes = p.ld_x * (k.f32 ? 4 : 2); k.gate_row_bytes = p.ld_x * 2; k.out_cols = p.n_in; k.depth = p.n_out;
     k.error_flags = error_flags;
     const uint32_t grid = tile_grid(p, p.n_in, t, sms);
-    if (t.cg == 2) return launch<kInputGrad, 256, 2>(a, b, k, grid, stream);
+    if (k.f32 && p.n_out > kChunk * kBK) return launch_long<kInputGrad>(a, b, k, t, grid, stream);
+    if (t.cg == 2) return launch<kInputGrad, 256, 2, false>(a, b, k, grid, stream);
     switch (t.bn) {
-    case 256: return launch<kInputGrad, 256, 1>(a, b, k, grid, stream);
-    case 128: return launch<kInputGrad, 128, 1>(a, b, k, grid, stream);
-    default: return launch<kInputGrad, 64, 1>(a, b, k, grid, stream);
+    case 256: return launch<kInputGrad, 256, 1, false>(a, b, k, grid, stream);
+    case 128: return launch<kInputGrad, 128, 1, false>(a, b, k, grid, stream);
+    default: return launch<kInputGrad, 64, 1, false>(a, b, k, grid, stream);
     }
 }
 
@@ -667,7 +780,7 @@ namespace {
 template <int BN, int CG>
 const char* weight_grad(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& k, const WeightGradPlan& w, cudaStream_t stream) {
     if (w.grid) {
-        const char* why = launch<kWeightGrad, BN, CG>(a, b, k, w.grid, stream);
+        const char* why = launch<kWeightGrad, BN, CG, true>(a, b, k, w.grid, stream);
         if (why) return why;
     }
     // Few tiles: all of them, and eight threads to a quad (each tile may have many partial sums); many tiles: the boundaries.

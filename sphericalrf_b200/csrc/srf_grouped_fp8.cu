@@ -44,19 +44,6 @@ template <int BN, int CG> __host__ __device__ constexpr int smem_bytes() {
     return b < kSmemMin ? kSmemMin : b;
 }
 
-// Registers of the 256-wide tile: 128 sums and two pieces of 32 in flight per scaling thread.  The block is launched with
-// 168 a thread (64512); 128 x 64 + 256 x 216 = 63488.
-constexpr int kRegsIssue = 64, kRegsScale = 216;
-static_assert(128 * kRegsIssue + 256 * kRegsScale <= kThreads * 168, "a larger share would wait for registers forever");
-
-__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) { return (uint64_t)lo | (uint64_t)hi << 32; }
-// Two fused multiply-adds, each rounded once.
-__device__ __forceinline__ void fma2(uint64_t& sum, uint64_t a, uint64_t b) {
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum) : "l"(a), "l"(b));
-}
-__device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
-
 // Copies of one lane's own values into shared memory, in groups that complete in order.
 __device__ __forceinline__ void copy_async4(float* dst, const float* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(smem_u32(dst)), "l"(src) : "memory");
@@ -120,7 +107,7 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     };
 
     if (warp < 4) {
-        if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsIssue));
+        if (BN == 256) regs_for_issue();
         if (warp == 0) {
             // ---- operand loads: one thread ----
             const uint32_t lead_full = CG == 2 ? leader_addr(bar_full) : bar_full;
@@ -182,7 +169,7 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         }
     } else {
         // ---- scale, sum, store ----
-        if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kRegsScale));
+        if (BN == 256) regs_for_sums();
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         unsigned char* stage = sm_store + (warp - 4) * 4096;
         const uint32_t lead_acc_empty = CG == 2 ? leader_addr(bar_acc_empty) : bar_acc_empty;

@@ -453,5 +453,23 @@ __device__ __forceinline__ void store_rows(const RowStore& s, const unsigned cha
     store_rows<false>(s, stage, none);
 }
 
+// ---- sums kept in registers, two to a 64-bit register ----
+
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) { return (uint64_t)lo | (uint64_t)hi << 32; }
+__device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+// Two fused multiply-adds, or two additions, each rounded once.
+__device__ __forceinline__ void fma2(uint64_t& sum, uint64_t a, uint64_t b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ void add2(uint64_t& sum, uint64_t a) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum) : "l"(a)); }
+
+// Registers of kernels whose 8 epilogue warps hold 128 sums a thread beside two pieces of 32 in flight.  A block of 384 is
+// launched with 168 a thread (64512).
+constexpr int kRegsIssue = 64, kRegsSum = 216;
+static_assert(128 * kRegsIssue + 256 * kRegsSum <= 384 * 168, "a larger share would wait for registers forever");
+__device__ __forceinline__ void regs_for_issue() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsIssue)); }
+__device__ __forceinline__ void regs_for_sums() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kRegsSum)); }
+
 }  // namespace tile
 }  // namespace srf

@@ -2,6 +2,7 @@
 
 Bounds, per output, from the arithmetic alone.  With T = sum |terms| of the exact sum and K its length:
   * fp32 accumulation in any order, also one that truncates: at most K 2^-23 T (one step of 2^-23 per addition);
+    Sums of fp32 results are cut into runs of 512 terms at most, which are added with rounding: (512 + K / 512) 2^-23 T;
   * rounding to the output type: half a step, eps/2 |y| (2^-11 fp16, 2^-8 bf16, 2^-24 fp32), and at least half of fp16's
     smallest step, 2^-25;
   * 8-bit layers: products of 8-bit values are exact in fp32; each block's scale is one rounded product (2^-24) and each
@@ -72,6 +73,11 @@ class Case:
         return abi.make_grouped(len(self.sizes), self.n_rows, self.n_in, self.n_out, self.type_id, out_id, **base)
 
 
+def fp32_length(terms):
+    """The K of the bound for a sum of `terms` products with an fp32 result."""
+    return min(terms, 512) + terms // 512 + 1
+
+
 def check_rows(got, exact, terms, length, used, where, buf, cols):
     """Rows of `used` within the bound; every other element of the buffer still POISON."""
     a, b = used
@@ -98,7 +104,7 @@ def run_layer(r, c, out, relu=False, stream=None):
         terms[a - c.used[0]:b - c.used[0]] = x.abs() @ w.abs().t()
     if relu:
         exact = exact.clamp_min(0)
-    check_rows(y, exact, terms, c.n_in, c.used, "layer", yb, c.n_out)
+    check_rows(y, exact, terms, fp32_length(c.n_in) if out == "f32" else c.n_in, c.used, "layer", yb, c.n_out)
     return y
 
 
@@ -115,7 +121,7 @@ def run_input_grad(r, c, out, gate=False):
         terms[a - c.used[0]:b - c.used[0]] = dy.abs() @ w.abs()
     if gate:
         exact = torch.where(c.x[c.used[0]:c.used[1]].double() > 0, exact, 0.0)
-    check_rows(dx, exact, terms, c.n_out, c.used, "input grad", dxb, c.n_in)
+    check_rows(dx, exact, terms, fp32_length(c.n_out) if out == "f32" else c.n_out, c.used, "input grad", dxb, c.n_in)
 
 
 def run_weight_grad(r, c, out):
@@ -129,7 +135,7 @@ def run_weight_grad(r, c, out):
     for g, (a, b) in enumerate(c.spans):
         dy, x = c.dy[a:b].double(), c.x[a:b].double()
         exact, terms = dy.t() @ x, dy.abs().t() @ x.abs()
-        bound = HALF_STEP[dt] * exact.abs() + TINY[dt] + (1 + HALF_STEP[dt]) * (b - a + 300) * 2.0 ** -23 * terms   # + joins of at most 2 x 148 partial sums
+        bound = HALF_STEP[dt] * exact.abs() + TINY[dt] + (1 + HALF_STEP[dt]) * (fp32_length(b - a) + 300) * 2.0 ** -23 * terms   # + joins of at most 2 x 148 partial sums
         if a == b:
             bound = torch.zeros_like(bound)
         bad = ~((dw[g].double() - exact).abs() <= bound)
@@ -177,6 +183,29 @@ def test_input_grad(r, shape, kind, out, gate):
 def test_weight_grad(r, shape, kind, out):
     sizes, n_in, n_out, front, back = SHAPES[shape]
     run_weight_grad(r, Case(sizes, n_in, n_out, kind, 90 + shape, front, back), out)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_long_sums_keep_fp32(r, kind):
+    """fp32 results of long sums, in the 2-norm.  An instruction adds 16 products to its accumulator and loses at most one
+    step of 2^-23 of it, half a step on average: 32 instructions of a run of 512 lose 32 2^-24 of the run's size, and the
+    runs' sizes and errors both add in squares, whatever their number."""
+    c = Case([700, 0, 9000], 4096, 1536, kind, 77)
+    y = torch.zeros(c.n_rows, c.n_out, device="cuda")
+    dx = torch.zeros(c.n_rows, c.n_in, device="cuda")
+    dw = torch.zeros(3, c.n_out, c.n_in, device="cuda")
+    r.grouped_matmul_device(c.layer(abi.TYPE_F32), c.offsets, c.x, c.w, y)
+    r.grouped_input_grad_device(c.layer(abi.TYPE_F32), c.offsets, c.dy, c.w, None, dx)
+    p = c.layer(abi.TYPE_F32)
+    space = torch.empty(r.grouped_weight_grad_workspace(p), dtype=torch.uint8, device="cuda")
+    r.grouped_weight_grad_device(p, c.offsets, c.dy, c.x, dw, space)
+    torch.cuda.synchronize()
+    for g, (a, b) in enumerate(c.spans):
+        if a == b:
+            continue
+        x, w, dy = c.x[a:b].double(), c.w[g].double(), c.dy[a:b].double()
+        for got, exact in ((y[a:b], x @ w.t()), (dx[a:b], dy @ w), (dw[g], dy.t() @ x)):
+            assert float((got.double() - exact).norm()) <= 32 * 2.0 ** -24 * float(exact.norm())
 
 
 def test_nan_of_one_group_stays_there(r):
