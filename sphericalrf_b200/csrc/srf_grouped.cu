@@ -69,12 +69,15 @@ template <int BN, int CG> __host__ __device__ constexpr int smem_bytes() {
     return b < kSmemMin ? kSmemMin : b;
 }
 
-// Units of work of a group: whole output tiles for the first two products; 64-sample stages of output tiles for the
-// weight gradient, whose work is cut evenly across the CTAs (see below).
+// Units of work of a group: whole output tiles for the first two products; for the weight gradient, whose work is cut evenly
+// across the CTAs (see below), the 64-sample stages of an output tile and kTileUnits in front of them, for what a tile costs
+// beside its stages: counted without, groups of few samples -- many shallow tiles -- held their CTAs up (both gradients of
+// 16389 x 2048 x 2048 in groups of 200 to 5000 samples: 324 us, with 4 units 307, 8 304, 14 302).
+constexpr uint32_t kTileUnits = 14;
 template <int MODE, int CG>
 __device__ __forceinline__ uint32_t group_units(const Span& s, uint32_t tiles_across) {
     const uint32_t rows = s.end - s.begin;
-    return (MODE == kWeightGrad ? (rows + kBK - 1) / kBK : (rows + CG * kBM - 1) / (CG * kBM)) * tiles_across;
+    return (MODE == kWeightGrad ? (rows ? (rows + kBK - 1) / kBK + kTileUnits : 0u) : (rows + CG * kBM - 1) / (CG * kBM)) * tiles_across;
 }
 
 // One stretch of summed stages of one output tile.
@@ -120,41 +123,45 @@ struct Pieces {
         }
     }
     __device__ __forceinline__ bool next(const GroupedArgs& p, uint32_t tiles_m, uint32_t tiles_n, Piece* o, bool* bad) {
-        if (MODE == kWeightGrad) {
-            while (at >= stop) {
-                worker += gridDim.x / CG;
-                if (worker >= p.n_workers) return false;
-                at = first_unit(units, worker, p.n_workers);
-                stop = first_unit(units, worker + 1, p.n_workers);
-            }
-        }
         const uint32_t across = MODE == kWeightGrad ? tiles_m * tiles_n : tiles_n;
-        uint32_t local;
-        if (!walk.find(at, p.offsets, p.n_groups, p.n_rows, [&](const Span& s) { return group_units<MODE, CG>(s, across); },
-                       &o->group, &o->span, &local, bad))
-            return false;
-        const uint32_t rows = o->span.end - o->span.begin;
-        uint32_t m;
-        if (MODE == kWeightGrad) {
-            const uint32_t deep = (rows + kBK - 1) / kBK;
-            const uint32_t t = local / deep;
-            tile_place(t, tiles_m, tiles_n, &m, &o->n);
-            o->m = m * (CG * kBM);
-            o->k0 = local - t * deep;
-            o->k_stages = deep - o->k0 < stop - at ? deep - o->k0 : stop - at;
-            o->first = o->k0 == 0;
-            o->whole = o->k_stages == deep;
-            o->worker = worker;
-            at += o->k_stages;
-        } else {
-            tile_place(local, (rows + CG * kBM - 1) / (CG * kBM), tiles_n, &m, &o->n);
-            o->m = o->span.begin + m * (CG * kBM);
-            o->k0 = 0;
-            o->k_stages = (p.depth + kBK - 1) / kBK;
-            o->first = o->whole = true;
-            at += step;
+        for (;;) {
+            if (MODE == kWeightGrad) {
+                while (at >= stop) {
+                    worker += gridDim.x / CG;
+                    if (worker >= p.n_workers) return false;
+                    at = first_unit(units, worker, p.n_workers);
+                    stop = first_unit(units, worker + 1, p.n_workers);
+                }
+            }
+            uint32_t local;
+            if (!walk.find(at, p.offsets, p.n_groups, p.n_rows, [&](const Span& s) { return group_units<MODE, CG>(s, across); },
+                           &o->group, &o->span, &local, bad))
+                return false;
+            const uint32_t rows = o->span.end - o->span.begin;
+            uint32_t m;
+            if (MODE == kWeightGrad) {
+                const uint32_t deep = (rows + kBK - 1) / kBK, cost = deep + kTileUnits;
+                const uint32_t t = local / cost, v = local - t * cost;
+                const uint32_t end = cost - v < stop - at ? cost : v + (stop - at);        // units of the tile up to which this worker goes
+                at += end - v;
+                if (end <= kTileUnits) continue;                                          // none of its stages
+                tile_place(t, tiles_m, tiles_n, &m, &o->n);
+                o->m = m * (CG * kBM);
+                o->k0 = v > kTileUnits ? v - kTileUnits : 0;
+                o->k_stages = end - kTileUnits - o->k0;
+                o->first = o->k0 == 0;
+                o->whole = o->k_stages == deep;
+                o->worker = worker;
+            } else {
+                tile_place(local, (rows + CG * kBM - 1) / (CG * kBM), tiles_n, &m, &o->n);
+                o->m = o->span.begin + m * (CG * kBM);
+                o->k0 = 0;
+                o->k_stages = (p.depth + kBK - 1) / kBK;
+                o->first = o->whole = true;
+                at += step;
+            }
+            return true;
         }
-        return true;
     }
 };
 
@@ -560,7 +567,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_weight_grad_join(const Grouped
             } else {
                 const uint32_t q = all / n, r = all - q * n;
                 auto owner = [&](uint32_t u) { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; };
-                const uint32_t u0 = before + t * deep, a = owner(u0), b = owner(u0 + deep - 1);
+                const uint32_t u0 = before + t * (deep + kTileUnits) + kTileUnits, a = owner(u0), b = owner(u0 + deep - 1);
                 if (a < b) { v0 = a; v1 = b; }
             }
         } else {
@@ -569,10 +576,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_weight_grad_join(const Grouped
             GroupWalk walk;
             Span s = {0, 0};
             if (u > 0 && u < units && walk.find(u, p.offsets, p.n_groups, p.n_rows, units_of, &group, &s, &local, &bad)) {
-                const uint32_t deep = (s.end - s.begin + kBK - 1) / kBK, t = local / deep, k = local - t * deep;
-                const uint32_t u0 = u - k, before = first_unit(units, blockIdx.x, n);
-                // the boundary cuts the tile, and the one in front of it does not
-                if (k > 0 && before <= u0 && before < u) {
+                const uint32_t deep = (s.end - s.begin + kBK - 1) / kBK, t = local / (deep + kTileUnits);
+                const uint32_t u0 = u - (local - t * (deep + kTileUnits)) + kTileUnits, before = first_unit(units, blockIdx.x, n);
+                // the boundary cuts the tile's stages (the first of which is unit u0), and the one in front of it does not
+                if (u > u0 && before <= u0) {
                     v0 = blockIdx.x;
                     v1 = v0 + 1;
                     while (v1 + 1 < n && first_unit(units, v1 + 1, n) < u0 + deep) ++v1;
@@ -629,7 +636,8 @@ WeightGradPlan plan_weight_grad(const srf_grouped_t& p, int sms) {
     w.cg = p.n_out > 128 && p.n_in > 128 ? 2 : 1;
     w.bn = p.n_in <= 64 ? 64 : p.n_in <= 128 ? 128 : 256;
     w.across = (uint64_t)((p.n_out + w.cg * kBM - 1) / (w.cg * kBM)) * ((p.n_in + w.bn - 1) / w.bn);
-    const uint64_t units = max_row_tiles(p, kBK) * w.across, teams = sms / w.cg;
+    const uint64_t filled = p.n_groups < p.n_rows ? p.n_groups : p.n_rows;
+    const uint64_t units = (max_row_tiles(p, kBK) + filled * kTileUnits) * w.across, teams = sms / w.cg;
     const uint64_t busy = units < teams ? units : teams;
     // All teams together walk the samples once per tile of a group that a team works on; samples beyond what L2 holds are
     // taken in two parts (16389 x 2048 x 2048 with its input gradient: 355 us in one, 305 in two, 310 in three, 329 in

@@ -118,8 +118,8 @@ inline std::string refuse_weight_grad_shape(const srf_grouped_t* in, srf_grouped
     const std::string why = refuse_grouped(in, kCallGradient, p);
     if (!why.empty()) return why;
     if (p->n_rows > (1ull << 26)) return "n_rows must be at most 2^26 for a weight gradient";
-    // the kernels count stages of 64 samples of 128 x 64 outputs (at the least) in 32 bits
-    if ((p->n_rows / 64 + p->n_groups) * ((p->n_out + 127ull) / 128) * ((p->n_in + 63ull) / 64) >= (1ull << 32)) return "n_rows x n_in x n_out is too large for one weight gradient";
+    // the kernels count stages of 64 samples of 128 x 64 outputs (at the least), and 14 a tile, in 32 bits
+    if ((p->n_rows / 64 + 15ull * p->n_groups) * ((p->n_out + 127ull) / 128) * ((p->n_in + 63ull) / 64) >= (1ull << 32)) return "n_rows x n_in x n_out is too large for one weight gradient";
     return "";
 }
 
