@@ -293,6 +293,11 @@ def test_bad_offsets_are_reported(r, offsets):
         with pytest.raises(abi.SrfError, match="offsets") as e:
             r.check_errors()
         assert e.value.status == abi.ERR_ARG
+    c8 = Case8([30, 30, 40], 64, 64, 9)
+    p = abi.make_grouped(3, c8.base.n_rows, 64, 64, abi.TYPE_E4M3, abi.TYPE_F16)
+    r.grouped_matmul_fp8_device(p, c.offsets, c8.x, c8.xs, c8.w, c8.ws, y[guard:])
+    with pytest.raises(abi.SrfError, match="offsets"):
+        r.check_errors()
     r.check_errors()
     assert bool((y[:guard] == POISON).all()) and bool((y[-guard:] == POISON).all())
     assert bool((dw[0] == POISON).all()) and bool((dw[4] == POISON).all())
@@ -341,6 +346,60 @@ def test_rows_behind_two_to_the_31_bytes_and_elements(r):
     for g, a, b in ((1, far, far + 150), (2, far + 150, far + 281)):
         exact, terms = x[a:b].double() @ w[g].double().t(), x[a:b].double().abs() @ w[g].double().abs().t()
         assert bool(((y[a:b].double() - exact).abs() <= 2.0 ** -11 * exact.abs() + 2.0 ** -25 + 1.001 * n_in * 2.0 ** -23 * terms).all())
+
+
+EXTREMES = [
+    ([k % 4 for k in range(4096)], 24, 16, 0, 1),          # the most groups
+    ([3], 16, 65536, 0, 0),                                # the widest layers
+    ([2, 1], 65536, 24, 0, 0),
+    ([5, 0, 2], 264, 520, 3, 200000),                      # a capacity far above what is used
+    ([1] * 148 * 3, 128, 256, 0, 0),                       # one sample a group
+]
+
+
+@pytest.mark.parametrize("case", range(len(EXTREMES)))
+def test_extremes(r, case):
+    sizes, n_in, n_out, front, back = EXTREMES[case]
+    c = Case(sizes, n_in, n_out, "f16", 300 + case, front, back)
+    run_layer(r, c, "f16", True)
+    run_layer(r, c, "f32")
+    run_input_grad(r, c, "f16", True)
+    run_weight_grad(r, c, "f32")
+    run_layer_fp8(r, Case8(sizes, n_in, n_out, 310 + case, front, back), "bf16", False)
+
+
+def test_calls_see_each_other(r):
+    """Calls set themselves up while the one in front still runs: a long chain without waits, torch's own kernels in
+    between, has the bits of the same chain with a wait after every step."""
+    n, off = 5000, torch.tensor([0, 1200, 1200, 5000], device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    w = (torch.randn(3, 64, 64, generator=gen, device="cuda") / 6).half()
+    start = torch.randn(n, 64, generator=gen, device="cuda").half()
+    fwd = abi.make_grouped(3, n, 64, 64, abi.TYPE_F16, activation=abi.ACT_RELU)
+    bwd, bww = abi.make_grouped(3, n, 64, 64, abi.TYPE_F16), abi.make_grouped(3, n, 64, 64, abi.TYPE_F16, abi.TYPE_F32)
+    space = torch.empty(r.grouped_weight_grad_workspace(bww), dtype=torch.uint8, device="cuda")
+
+    def chain(wait):
+        a, b, d = start.clone(), torch.zeros_like(start), torch.zeros_like(start)
+        dw, total = torch.zeros(3, 64, 64, device="cuda"), torch.zeros(3, 64, 64, device="cuda")
+        q, qs = torch.zeros(n, 64, dtype=torch.uint8, device="cuda"), torch.zeros(1, n, device="cuda")
+        for i in range(30):
+            r.grouped_matmul_device(fwd, off, a, w, b)
+            wait()
+            r.grouped_input_grad_device(bwd, off, b, w, b.clone() if i % 3 == 0 else None, d)
+            wait()
+            r.grouped_weight_grad_device(bww, off, d, b, dw, space)
+            wait()
+            r.quantize_rows_device(abi.TYPE_F16, n, 64, d, 64, q, 64, qs)
+            wait()
+            total += dw
+            a.copy_(d).mul_(0.5).add_(q.view(torch.float8_e4m3fn).half(), alpha=0.001).clamp_(-4, 4)
+            wait()
+        torch.cuda.synchronize()
+        return a, total, q, qs
+
+    for got, want in zip(chain(lambda: None), chain(torch.cuda.synchronize)):
+        assert torch.equal(got, want)
 
 
 # ---- 8 bits ----
@@ -455,10 +514,14 @@ class Case8:
 @pytest.mark.parametrize("shape", range(len(SHAPES)))
 def test_layer_fp8(r, shape, out, relu):
     sizes, n_in, n_out, front, back = SHAPES[shape]
-    c = Case8(sizes, n_in, n_out, 200 + shape, front, back)
+    run_layer_fp8(r, Case8(sizes, n_in, n_out, 200 + shape, front, back), out, relu)
+
+
+def run_layer_fp8(r, c, out, relu):
+    n_in, n_out = c.n_in, c.n_out
     out_id, dt = TYPES[out]
     yb, y = table(c.base.n_rows, n_out, dt, 8, POISON)
-    p = abi.make_grouped(len(sizes), c.base.n_rows, n_in, n_out, abi.TYPE_E4M3, out_id, abi.ACT_RELU if relu else abi.ACT_NONE,
+    p = abi.make_grouped(len(c.base.sizes), c.base.n_rows, n_in, n_out, abi.TYPE_E4M3, out_id, abi.ACT_RELU if relu else abi.ACT_NONE,
                          c.xb.stride(0), c.wb.stride(1), yb.stride(0), c.wb.stride(0))
     r.grouped_matmul_fp8_device(p, c.base.offsets, c.x, c.xs, c.w, c.ws, y)
     torch.cuda.synchronize()
