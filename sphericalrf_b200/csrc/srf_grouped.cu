@@ -14,7 +14,9 @@
 // tiles itself from the offsets (GroupWalk), so no launch, workspace or host read prepares them.
 //
 // Large layers run on pairs of CTAs (CG = 2): one instruction computes 256 x 256 outputs on two SMs, each of which
-// loads its own 128 rows of A and half of B, so that an operand byte from L2 serves twice as many products.
+// loads its own 128 rows of A and half of B, so that an operand byte from L2 serves twice as many products.  Their tiles
+// are 160 to 256 columns wide, in steps of 32, so that the columns divide evenly: 656 columns are three tiles of 224 (66
+// groups of 1057 samples, 780 -> 656: 84.7 us against 88.7).
 //
 // The tensor core's additions to an accumulator truncate, so that a long sum's error grows with its length (2-norm 2.1e-6 at
 // 2048 products, 9e-6 at 8192, where fp32 additions one by one have 4e-7): nothing beside a rounding to 16 bits, but not
@@ -56,6 +58,7 @@ struct GroupedArgs {
     uint32_t out_rows;            // weight gradient: n_out
     uint32_t out_cols;            // n_out, n_in, n_in
     uint32_t depth;               // summed length of the first two products
+    uint32_t width;               // columns of a pair's tile
     uint32_t n_workers;           // weight gradient: even shares of the work
     int bf16, f32, relu;
     unsigned int* error_flags;
@@ -203,7 +206,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const uint32_t bar_tail = bar_acc_empty + 8 * kAccs;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;
-    const uint32_t tiles_n = (p.out_cols + BN - 1) / BN;
+    const uint32_t width = CG == 2 ? p.width : BN;                 // columns of a tile
+    const uint32_t tiles_n = (p.out_cols + width - 1) / width;
     const uint32_t tiles_m = MODE == kWeightGrad ? (p.out_rows + CG * kBM - 1) / (CG * kBM) : 0;
 
     // Barriers of a pair: `full` and `acc_empty` are those of rank 0, where the instructions are issued; `empty` and
@@ -240,13 +244,13 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             Ring<kStages> at;
             uint32_t issued = 0, tails = 0;
             while (ok && pieces.next(p, tiles_m, tiles_n, &t, &bad)) {
-                const int am = (int)(t.m + rank * kBM), bn = (int)(t.n * BN + rank * kBRows);
+                const int am = (int)(t.m + rank * kBM), bn = (int)(t.n * width + rank * (width / CG));
                 // weight gradient: the group's last stage, if it is of this piece and not a full one
                 const uint32_t deep = t.span.end - t.span.begin;
                 const bool tail = MODE == kWeightGrad && (t.k0 + t.k_stages) * kBK > deep;
                 // single CTAs load only the rows that the group has (what lies in the others' place is never stored)
                 const uint32_t boxes = MODE == kWeightGrad || CG == 2 || t.span.end - t.m >= (uint32_t)kBM ? kBM / kRowBox : (t.span.end - t.m + kRowBox - 1) / kRowBox;
-                const uint32_t bytes = boxes * (kABytes / (kBM / kRowBox)) + kBBytes;
+                const uint32_t bytes = boxes * (kABytes / (kBM / kRowBox)) + (MODE == kLayer ? width / CG * (kBK * 2) : kBBytes);
                 if (elect_one()) {
                     Ring<kStages> r = at;
                     for (uint32_t k = 0; k < t.k_stages; ++k) {
@@ -298,7 +302,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             if ((!ok || *failed) && rank == 0) drain_ring<kStages>(bar_full, issued);
         } else if (warp == 1 && rank == 0) {
             // ---- matrix instructions: one thread ----
-            const uint32_t idesc = idesc_shape(CG * kBM, BN) | (p.bf16 ? (1u << 7) | (1u << 10) : 0u) | (kAColumns ? 1u << 15 : 0u) | (kBColumns ? 1u << 16 : 0u);
+            const uint32_t idesc = idesc_shape(CG * kBM, width) | (p.bf16 ? (1u << 7) | (1u << 10) : 0u) | (kAColumns ? 1u << 15 : 0u) | (kBColumns ? 1u << 16 : 0u);
             const uint64_t desc_a = operand_desc(smem_u32(sm_a), kAColumns ? 8192 : 16, 1024), desc_b = operand_desc(smem_u32(sm_b), kBColumns ? 8192 : 16, 1024);
             constexpr uint32_t kStepA = kAColumns ? 2048 : 32, kStepB = kBColumns ? 2048 : 32;      // bytes of 16 summed indices
             Ring<kStages> at;
@@ -373,7 +377,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             if (!ok) break;
             const bool partial = MODE == kWeightGrad && !t.whole;
             const uint32_t row0 = t.m + rank * kBM + quarter * 32, end = MODE == kWeightGrad ? p.out_rows : t.span.end;
-            const uint32_t col0 = t.n * BN + half * kCols;
+            const uint32_t col0 = t.n * width + half * kCols, room = width - half * kCols;      // 32 columns at least
             RowStore rs;
             rs.bf16 = p.bf16 != 0;
             rs.f32 = partial || p.f32;
@@ -390,7 +394,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 out = p.out + (MODE == kWeightGrad ? t.group * p.out_group_bytes : 0ull) + row0 * p.out_row_bytes + (size_t)col0 * (rs.f32 ? 4 : 2);
                 rs.row_bytes = p.out_row_bytes;
             }
-            const uint32_t cols = col0 >= p.out_cols ? 0u : p.out_cols - col0 < (uint32_t)kCols ? p.out_cols - col0 : (uint32_t)kCols;
+            const uint32_t cols = col0 >= p.out_cols ? 0u : min(min(p.out_cols - col0, (uint32_t)kCols), room);
             if (rs.f32) {
 #pragma unroll
                 for (int c = 0; c < kCols; c += 32) {
@@ -448,8 +452,8 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             rs.f32 = p.f32;
             const uint32_t row0 = t.m + rank * kBM + quarter * 32;
             rs.rows = row0 >= t.span.end ? 0u : t.span.end - row0 < 32 ? t.span.end - row0 : 32u;
-            const uint32_t col0 = t.n * BN;
-            const uint32_t cols = p.out_cols - col0 < (uint32_t)BN ? p.out_cols - col0 : (uint32_t)BN;
+            const uint32_t col0 = t.n * width;
+            const uint32_t cols = p.out_cols - col0 < width ? p.out_cols - col0 : width;
             unsigned char* out = p.out + row0 * p.out_row_bytes;
             rs.row_bytes = p.out_row_bytes;
             const uint32_t per = rs.f32 ? 32u : 64u, size = rs.f32 ? 4u : 2u;
@@ -526,7 +530,8 @@ template <int BN, int CG, int LANES> __host__ __device__ constexpr int join_slic
 template <int BN, int CG, int LANES, bool BY_TILE>
 __global__ void __launch_bounds__(kJoinThreads) k_weight_grad_join(const GroupedArgs p) {
     constexpr uint32_t kSlices = join_slices<BN, CG, LANES>(), kQuads = CG * kBM * BN / 4 / kSlices;
-    const uint32_t tiles_n = (p.out_cols + BN - 1) / BN, tiles_m = (p.out_rows + CG * kBM - 1) / (CG * kBM);
+    const uint32_t width = CG == 2 ? p.width : BN;
+    const uint32_t tiles_n = (p.out_cols + width - 1) / width, tiles_m = (p.out_rows + CG * kBM - 1) / (CG * kBM);
     const uint32_t across = tiles_m * tiles_n, slice = blockIdx.y, n = p.n_workers;
     wait_for_inputs();
     let_next_start();
@@ -594,8 +599,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_weight_grad_join(const Grouped
     if (v0 > v1 && !empty) return;
     for (uint32_t i = threadIdx.x / LANES; i < kQuads; i += kJoinThreads / LANES) {
         const uint32_t at = slice * kQuads + i, row = at / (BN / 4), col = at % (BN / 4) * 4;
-        const uint32_t orow = sh[3] * (CG * kBM) + row, ocol = sh[4] * BN + col;
-        const bool inside = orow < p.out_rows && ocol < p.out_cols;
+        const uint32_t orow = sh[3] * (CG * kBM) + row, ocol = sh[4] * width + col;
+        const bool inside = orow < p.out_rows && ocol < p.out_cols && col < width;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         if (inside && !empty) {
             const float4* q = reinterpret_cast<const float4*>(p.partial + (size_t)row * BN + col);
@@ -629,13 +634,20 @@ __global__ void __launch_bounds__(kJoinThreads) k_weight_grad_join(const Grouped
     }
 }
 
+// Width of a pair's tiles: as many tiles as 256 columns each would make, evenly.
+uint32_t pair_width(uint32_t cols) {
+    const uint32_t tiles = (cols + 255) / 256, even = ((cols + tiles - 1) / tiles + 31) / 32 * 32;
+    return even < 160 ? 160 : even;
+}
+
 // Shape and shares of the weight gradient.
-struct WeightGradPlan { int bn, cg; uint64_t across; uint32_t grid, workers; };
+struct WeightGradPlan { int bn, cg; uint32_t width; uint64_t across; uint32_t grid, workers; };
 WeightGradPlan plan_weight_grad(const srf_grouped_t& p, int sms) {
     WeightGradPlan w;
     w.cg = p.n_out > 128 && p.n_in > 128 ? 2 : 1;
     w.bn = p.n_in <= 64 ? 64 : p.n_in <= 128 ? 128 : 256;
-    w.across = (uint64_t)((p.n_out + w.cg * kBM - 1) / (w.cg * kBM)) * ((p.n_in + w.bn - 1) / w.bn);
+    w.width = w.cg == 2 ? pair_width(p.n_in) : w.bn;
+    w.across = (uint64_t)((p.n_out + w.cg * kBM - 1) / (w.cg * kBM)) * ((p.n_in + w.width - 1) / w.width);
     const uint64_t filled = p.n_groups < p.n_rows ? p.n_groups : p.n_rows;
     const uint64_t units = (max_row_tiles(p, kBK) + filled * kTileUnits) * w.across, teams = sms / w.cg;
     const uint64_t busy = units < teams ? units : teams;
@@ -673,9 +685,9 @@ uint64_t max_row_tiles(const srf_grouped_t& p, uint64_t height) {
     return p.n_rows / height + busy;
 }
 
-TileShape pick_tile(const srf_grouped_t& p, uint32_t cols, int sms, int smallest) {
+TileShape pick_tile(const srf_grouped_t& p, uint32_t cols, int sms, int smallest, int cols_step) {
     // Pairs: groups of a few 256-row tiles at least, and enough tiles for every pair.
-    if (cols > 128 && p.n_rows / p.n_groups >= 512 && p.n_rows / 256 * ((cols + 255) / 256) >= (uint64_t)sms) return {256, 2};
+    if (cols > 128 && p.n_rows / p.n_groups >= 512 && p.n_rows / 256 * ((cols + 255) / 256) >= (uint64_t)sms) return {cols_step == 32 ? (int)pair_width(cols) : 256, 2};
     // Otherwise the width that costs least: rounds of tiles over the SMs, times a tile's share of loads -- its columns, its
     // samples, and as much as 32 columns for what every tile costs.
     const uint64_t busy = p.n_groups < p.n_rows ? p.n_groups : p.n_rows;
@@ -732,7 +744,7 @@ const char* launch_grouped_matmul(const srf_grouped_t& p, const uint64_t* offset
                                   unsigned int* error_flags, cudaStream_t stream) {
     if (!p.n_rows) return nullptr;
     const int sms = sm_count();
-    const TileShape t = pick_tile(p, p.n_out, sms, p.out_type == SRF_TYPE_F32 && p.n_in > kChunk * kBK ? 64 : 32);
+    const TileShape t = pick_tile(p, p.n_out, sms, p.out_type == SRF_TYPE_F32 && p.n_in > kChunk * kBK ? 64 : 32, 32);
     CUtensorMap a, b;
     if (!make_operand_map(&a, x, p.type, p.n_in, p.n_rows, p.ld_x, 0, 0, t.cg == 2 ? kBM : kRowBox) ||
         !make_operand_map(&b, w, p.type, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, t.bn / t.cg))
@@ -741,7 +753,7 @@ const char* launch_grouped_matmul(const srf_grouped_t& p, const uint64_t* offset
     memset(&k, 0, sizeof(k));
     k.offsets = offsets; k.out = (unsigned char*)y; k.n_rows = (uint32_t)p.n_rows; k.n_groups = p.n_groups;
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16; k.relu = p.activation == SRF_ACT_RELU;
-    k.out_row_bytes = p.ld_y * (k.f32 ? 4 : 2); k.out_cols = p.n_out; k.depth = p.n_in; k.error_flags = error_flags;
+    k.out_row_bytes = p.ld_y * (k.f32 ? 4 : 2); k.out_cols = p.n_out; k.depth = p.n_in; k.width = t.bn; k.error_flags = error_flags;
     const uint32_t grid = tile_grid(p, p.n_out, t, sms);
     if (k.f32 && p.n_in > kChunk * kBK) return launch_long<kLayer>(a, b, k, t, grid, stream);
     if (t.cg == 2) return launch<kLayer, 256, 2, false>(a, b, k, grid, stream);
@@ -757,7 +769,7 @@ const char* launch_grouped_input_grad(const srf_grouped_t& p, const uint64_t* of
                                       const void* gate, void* dx, unsigned int* error_flags, cudaStream_t stream) {
     if (!p.n_rows) return nullptr;
     const int sms = sm_count();
-    const TileShape t = pick_tile(p, p.n_in, sms, 64);
+    const TileShape t = pick_tile(p, p.n_in, sms, 64, 32);
     CUtensorMap a, b;
     if (!make_operand_map(&a, dy, p.type, p.n_out, p.n_rows, p.ld_y, 0, 0, t.cg == 2 ? kBM : kRowBox) ||
         !make_operand_map(&b, w, p.type, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, kBK))
@@ -766,7 +778,7 @@ const char* launch_grouped_input_grad(const srf_grouped_t& p, const uint64_t* of
     memset(&k, 0, sizeof(k));
     k.offsets = offsets; k.out = (unsigned char*)dx; k.gate = (const unsigned char*)gate; k.n_rows = (uint32_t)p.n_rows; k.n_groups = p.n_groups;
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16;
-    k.out_row_bytes = p.ld_x * (k.f32 ? 4 : 2); k.gate_row_bytes = p.ld_x * 2; k.out_cols = p.n_in; k.depth = p.n_out;
+    k.out_row_bytes = p.ld_x * (k.f32 ? 4 : 2); k.gate_row_bytes = p.ld_x * 2; k.out_cols = p.n_in; k.depth = p.n_out; k.width = t.bn;
     k.error_flags = error_flags;
     const uint32_t grid = tile_grid(p, p.n_in, t, sms);
     if (k.f32 && p.n_out > kChunk * kBK) return launch_long<kInputGrad>(a, b, k, t, grid, stream);
@@ -809,7 +821,7 @@ const char* launch_grouped_weight_grad(const srf_grouped_t& p, const uint64_t* o
     k.offsets = offsets; k.out = (unsigned char*)dw; k.partial = (float*)workspace; k.n_rows = (uint32_t)p.n_rows; k.n_groups = p.n_groups;
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16;
     k.out_row_bytes = p.ld_w * (k.f32 ? 4 : 2); k.out_group_bytes = p.group_stride * (k.f32 ? 4 : 2);
-    k.out_rows = p.n_out; k.out_cols = p.n_in; k.n_workers = w.workers; k.error_flags = error_flags;
+    k.out_rows = p.n_out; k.out_cols = p.n_in; k.width = w.width; k.n_workers = w.workers; k.error_flags = error_flags;
     CUtensorMap a, b;
     memset(&a, 0, sizeof(a));
     memset(&b, 0, sizeof(b));

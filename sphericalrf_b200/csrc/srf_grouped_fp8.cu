@@ -285,7 +285,7 @@ const char* launch_grouped_matmul_fp8(const srf_grouped_t& p, const uint64_t* of
                                       cudaStream_t stream) {
     if (!p.n_rows) return nullptr;
     const int sms = sm_count();
-    const TileShape t = pick_tile(p, p.n_out, sms, 64);
+    const TileShape t = pick_tile(p, p.n_out, sms, 64, 256);
     CUtensorMap a, b;
     if (!make_operand_map(&a, x, SRF_TYPE_E4M3, p.n_in, p.n_rows, p.ld_x, 0, 0, t.cg == 2 ? kBM : kRowBox) ||
         !make_operand_map(&b, w, SRF_TYPE_E4M3, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, t.bn / t.cg))

@@ -36,7 +36,8 @@ uint64_t max_row_tiles(const srf_grouped_t& p, uint64_t height);
 // loads its samples in boxes of kRowBox rows, as many as the tile has.
 constexpr uint32_t kRowBox = 32;
 struct TileShape { int bn, cg; };
-TileShape pick_tile(const srf_grouped_t& p, uint32_t cols, int sms, int smallest);
+// `cols_step`: 32 where a pair's tiles may be narrower than 256 (8-bit tiles may not: their halves are scale blocks).
+TileShape pick_tile(const srf_grouped_t& p, uint32_t cols, int sms, int smallest, int cols_step);
 // CTAs for them: one per SM, no more than there can be tiles.
 uint32_t tile_grid(const srf_grouped_t& p, uint32_t cols, TileShape t, int sms);
 

@@ -161,6 +161,7 @@ SHAPES = [
     ([9000, 30000], 700, 264, 0, 0),
     ([700, 90, 0, 1500, 64, 333, 1, 2000], 1100, 600, 0, 11),
     ([30] * 160 + [0] * 3 + [500, 7], 40, 72, 5, 0),
+    ([30000], 420, 170, 0, 0),
 ]
 
 
