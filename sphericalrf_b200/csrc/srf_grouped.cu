@@ -23,6 +23,10 @@
 // what a result in fp32 should have.  LONG kernels therefore start a new accumulator every 512 products and add those in
 // registers, rounded (5e-7 at any length); both sets of epilogue warps work on every tile then, half of its columns each.
 //
+// Measured (one B200): 32801 samples in 16 groups, 2048 -> 2043: 179 us alone (1.53 PFLOP/s, tensor pipe 93 %), 214-222 us a call
+// under the power limit (single CTAs 241); 160 samples in 64 groups, 2048 -> 1408: 63-67 us, 5.7 TB/s of matrices; 1048613
+// samples 32 -> 64: 40-42 us, 4.9 TB/s; weight gradient of 16389 x 2048 x 2048: 150 us alone and 35 for its joins.
+//
 // A tile's rows behind its group's end hold the next group's samples: harmless in the first two products (an output row
 // depends on its own sample alone and those rows are not stored).  In the weight gradient they would be summed, so the
 // rows of the last stage of a group are zeroed in shared memory, in both operands (a NaN of the next group must not

@@ -13,7 +13,7 @@
 // maximum is not finite is gone through again, value by value.
 //
 // Bound by memory: two bytes read, one written per value, one pass (the block stays in registers between the maximum
-// and the quotients).
+// and the quotients).  65539 x 2048: 70 us alone, 74-77 a call, 5.5 TB/s; 66 % of the issue slots are taken.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "srf_layers.cuh"
