@@ -25,7 +25,7 @@
 //
 // Measured (one B200): 32801 samples in 16 groups, 2048 -> 2043: 179 us alone (1.53 PFLOP/s, tensor pipe 93 %), 214-222 us a call
 // under the power limit (single CTAs 241); 160 samples in 64 groups, 2048 -> 1408: 63-67 us, 5.7 TB/s of matrices; 1048613
-// samples 32 -> 64: 40-42 us, 4.9 TB/s; weight gradient of 16389 x 2048 x 2048: 150 us alone and 35 for its joins.
+// samples 32 -> 64: 41-43 us, 4.8 TB/s; weight gradient of 16389 x 2048 x 2048: 150 us alone and 35 for its joins.
 //
 // A tile's rows behind its group's end hold the next group's samples: harmless in the first two products (an output row
 // depends on its own sample alone and those rows are not stored).  In the weight gradient they would be summed, so the

@@ -205,7 +205,7 @@ k_grouped_fp8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             }
             float sw_lane = 0.f;
             for (uint32_t k = 0; k < blocks_k; ++k) {
-                if ((k & 31) == 0) sw_lane = k + lane < blocks_k ? __ldg(sw + k + lane) : 0.f;
+                if ((k & 31) == 0) sw_lane = k + lane < blocks_k ? __ldcg(sw + k + lane) : 0.f;
                 copy_async_wait<kScaleAhead - 1>();
                 float* slot = ring + (k % kScaleAhead) * 32;
                 const float scale = *slot * __shfl_sync(0xffffffffu, sw_lane, k & 31);

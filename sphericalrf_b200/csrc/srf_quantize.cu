@@ -13,7 +13,7 @@
 // maximum is not finite is gone through again, value by value.
 //
 // Bound by memory: two bytes read, one written per value, one pass (the block stays in registers between the maximum
-// and the quotients).  65539 x 2048: 70 us alone, 74-77 a call, 5.5 TB/s; 66 % of the issue slots are taken.
+// and the quotients).  65539 x 2048: 70 us alone, 74-78 a call, 5.3 TB/s; 66 % of the issue slots are taken.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "srf_layers.cuh"
@@ -43,11 +43,11 @@ __device__ __forceinline__ void unpack8(uint4 v, bool bf16, float (&f)[8]) {
 
 // Eight values from `p`, of which `have` (0..8) exist; zeros behind them.
 __device__ __forceinline__ uint4 load8(const uint16_t* p, int have) {
-    if (have >= 8) return __ldg(reinterpret_cast<const uint4*>(p));
+    if (have >= 8) return __ldcg(reinterpret_cast<const uint4*>(p));
     uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (i < have) w[i >> 1] |= (uint32_t)__ldg(p + i) << ((i & 1) * 16);
+        if (i < have) w[i >> 1] |= (uint32_t)__ldcg(p + i) << ((i & 1) * 16);
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -145,7 +145,7 @@ k_quantize_rows(int bf16, uint64_t n_rows, const uint64_t* __restrict__ n_used, 
     uint64_t rows = n_rows;
     tile::wait_for_inputs();
     tile::let_next_start();
-    if (n_used) { const uint64_t u = __ldg((const unsigned long long*)n_used); rows = u < rows ? u : rows; }
+    if (n_used) { const uint64_t u = __ldcg((const unsigned long long*)n_used); rows = u < rows ? u : rows; }
     const int lane = threadIdx.x & 31;
     const uint32_t block = blockIdx.y * 2 + (lane >> 4);
     const uint64_t row0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * kRowsPerWarp;
@@ -158,7 +158,7 @@ k_quantize_rows(int bf16, uint64_t n_rows, const uint64_t* __restrict__ n_used, 
     out += row0 * ld_out;
     if (full) {
 #pragma unroll
-        for (int i = 0; i < kRowsPerWarp; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(in + i * ld_in + col));
+        for (int i = 0; i < kRowsPerWarp; ++i) v[i] = __ldcg(reinterpret_cast<const uint4*>(in + i * ld_in + col));
     } else {
 #pragma unroll
         for (int i = 0; i < kRowsPerWarp; ++i) v[i] = row0 + i < rows ? load8(in + i * ld_in + col, have) : make_uint4(0u, 0u, 0u, 0u);

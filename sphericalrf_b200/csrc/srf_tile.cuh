@@ -64,7 +64,8 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // Programmatic dependent launch: a kernel's blocks may be set up while the kernel in front of it in the stream still runs.
-// Nothing in global memory is touched in front of wait_for_inputs(), which returns when that kernel has completed.
+// Nothing in global memory is touched in front of wait_for_inputs(), which returns when that kernel has completed.  Loads
+// behind it go to L2 (__ldcg) or through TMA, never the read-only path: that may keep lines from the time before.
 __device__ __forceinline__ void wait_for_inputs() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -243,7 +244,7 @@ struct Span { uint32_t begin, end; };
 __device__ __forceinline__ Span group_span(const uint64_t* __restrict__ offsets, uint32_t g, uint32_t n_rows, bool* bad) {
     Span s = {0, n_rows};
     if (offsets) {
-        const uint64_t b = __ldg((const unsigned long long*)offsets + g), e = __ldg((const unsigned long long*)offsets + g + 1);
+        const uint64_t b = __ldcg((const unsigned long long*)offsets + g), e = __ldcg((const unsigned long long*)offsets + g + 1);
         if (b > e || e > n_rows) *bad = true;
         s.end = e < n_rows ? (uint32_t)e : n_rows;
         s.begin = b < s.end ? (uint32_t)b : s.end;
@@ -393,10 +394,10 @@ __device__ __forceinline__ void load_gate(const RowStore& s, uint4 (&hv)[8]) {
             const uint32_t have = s.bytes - from;
             if (have >= 16u) {
                 if (s.f32) {
-                    const uint2 t = __ldg(reinterpret_cast<const uint2*>(gp));
+                    const uint2 t = __ldcg(reinterpret_cast<const uint2*>(gp));
                     hv[it] = make_uint4(t.x, t.y, 0u, 0u);
                 } else {
-                    hv[it] = __ldg(reinterpret_cast<const uint4*>(gp));
+                    hv[it] = __ldcg(reinterpret_cast<const uint4*>(gp));
                 }
             } else {
                 const uint16_t* h = reinterpret_cast<const uint16_t*>(gp);
@@ -404,7 +405,7 @@ __device__ __forceinline__ void load_gate(const RowStore& s, uint4 (&hv)[8]) {
                 uint32_t t[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if ((uint32_t)e < n) t[e >> 1] |= (uint32_t)__ldg(h + e) << ((e & 1) * 16);
+                    if ((uint32_t)e < n) t[e >> 1] |= (uint32_t)__ldcg(h + e) << ((e & 1) * 16);
                 hv[it] = make_uint4(t[0], t[1], t[2], t[3]);
             }
         }
