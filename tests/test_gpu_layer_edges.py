@@ -1,0 +1,67 @@
+"""Edges of the layer operators beside those of test_gpu_layers.py, whose bounds and cases these tests use."""
+import pytest
+
+from sphericalrf_b200 import abi
+from test_gpu_layers import POISON, TYPES, Case8, check_rows, r, table, up  # noqa: F401  (r is the fixture)
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+def exponents(shape, low, high, seed):
+    """Scales of random mantissa between 2^low and 2^high."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.exp2(low + (high - low) * torch.rand(*shape, generator=gen, device="cuda", dtype=torch.float64)).float()
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("scales", ["small", "smaller", "subnormal", "large", "mixed", "zero"])
+@pytest.mark.parametrize("sizes,n_in,n_out", [([129, 127, 0, 1], 64, 64), ([300, 17, 64], 300, 500), ([9000, 30000], 700, 264)])
+def test_scales_whose_product_is_no_normal_number(r, sizes, n_in, n_out, scales, out):  # noqa: F811
+    """Two scales may be far from 1 where the results are ordinary numbers.  Their product may not be rounded to fewer bits,
+    vanish or become infinite on the way.  The bound is the one of every 8-bit layer: a block's sum meets two roundings, be
+    it by the product of the scales or by one after the other."""
+    c = Case8(sizes, n_in, n_out, 400, 2, 3)
+    a, b = c.base.used
+    big_x = (c.base.x[a:b].float() * 100).clamp(max=448).to(torch.float8_e4m3fn)
+    big_w = (c.base.w.float().abs() * n_in ** 0.5 * 100).clamp(max=448).to(torch.float8_e4m3fn)
+    xs, ws = c.xs[:, a:b].shape, c.ws.shape
+    if scales == "large":
+        # sums of at most 128 x 2^-8 x 2^-9 against a product of 2^128 to 2^132
+        c.x[a:b] = (2.0 ** -8 * (c.base.x[a:b].float() > 0.5).float()).to(torch.float8_e4m3fn)
+        c.w[:] = (2.0 ** -9 * c.base.w.float().sign()).to(torch.float8_e4m3fn)
+        c.xs[:, a:b], c.ws = exponents(xs, 116, 118, 1), exponents(ws, 12, 14, 2)
+    elif scales == "zero":
+        # a block of zeros whose scales' product is infinite: its term is 0
+        c.x[a:b, :128] = 0
+        c.xs[0, a:b], c.ws[:, :, 0] = 2.0 ** 118, 2.0 ** 118
+    else:
+        c.x[a:b], c.w[:] = big_x, big_w
+        low_x, low_w = {"small": (-126, -14), "smaller": (-82, -62), "subnormal": (-145, 8), "mixed": (-126, -14)}[scales]
+        c.xs[:, a:b], c.ws = exponents(xs, low_x, low_x + 4, 1), exponents(ws, low_w, low_w + 4, 2)
+        if scales == "mixed":
+            c.xs[:, a:b:2] = exponents(c.xs[:, a:b:2].shape, -4, 0, 3)
+    out_id, dt = TYPES[out]
+    yb, y = table(c.base.n_rows, n_out, dt, 8, POISON)
+    p = abi.make_grouped(len(sizes), c.base.n_rows, n_in, n_out, abi.TYPE_E4M3, out_id, abi.ACT_NONE, c.xb.stride(0), c.wb.stride(1), yb.stride(0), c.wb.stride(0))
+    r.grouped_matmul_fp8_device(p, c.base.offsets, c.x, c.xs, c.w, c.ws, y)
+    torch.cuda.synchronize()
+    exact, terms = c.exact()
+    assert bool((exact.abs() < 2.0 ** 127).all())
+    blocks = up(n_in, 128) // 128
+    check_rows(y, exact, terms, n_in + 2 * blocks + 2, c.base.used, scales, yb, n_out)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_scales_that_are_not_finite_stay_in_their_rows(r, bad):  # noqa: F811
+    c = Case8([100], 256, 96, 401)
+    c.x[:] = 1.0
+    c.w[:] = 1.0
+    c.xs[1, 40] = bad
+    y = torch.full((100, 96), POISON, device="cuda")
+    r.grouped_matmul_fp8_device(abi.make_grouped(1, 100, 256, 96, abi.TYPE_E4M3, abi.TYPE_F32), None, c.x, c.xs, c.w, c.ws, y)
+    torch.cuda.synchronize()
+    assert not bool(y[40].isfinite().any())
+    rest = torch.arange(100, device="cuda") != 40
+    exact, terms = c.exact()
+    assert bool(((y.double() - exact).abs() <= 1.001 * 262 * 2.0 ** -23 * terms)[rest].all())
