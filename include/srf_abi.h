@@ -456,12 +456,15 @@ srf_status srf_dump_samples(srf_ctx* ctx, const srf_view_t* view, uint64_t ray_f
                             float* h_pos_dt, uint32_t* h_ordinal, uint32_t* h_cell,
                             uint64_t* n_total);
 
-/* Device-side error word of the context (the reference has none: its kernels cannot time out).  Bits: 1 = a
-   ray hit the march loop's iteration bound, 2 = a wait on the tensor-core commit barrier expired, 4 = the
-   sample pool ran out of chunks, 16 = a layer call met offsets outside its buffers (reported as SRF_ERR_ARG).  Frames enqueued without `stats` do not synchronise and therefore cannot
-   report; the word stays set across frames until one of srf_render, srf_dump_samples, a frame with `stats`
-   or this call has returned it as SRF_ERR_TIMEOUT / SRF_ERR_CAPACITY, which also clears it.  Synchronises
-   `stream`.  `flags` (may be NULL) receives the raw word. */
+/* Device-side error words of the context (the reference has none: its kernels cannot time out).  Bits: 1 = a
+   ray hit the march loop's iteration bound, 2 = a bounded wait of a kernel expired, 4 = the sample pool ran out of
+   chunks, 8 = the fused grid refresh met a masked cell, 16 = a layer call met offsets outside its buffers.  Frames enqueued
+   without `stats` do not synchronise and therefore cannot report; their word stays set across frames until one of
+   srf_render, srf_dump_samples, a frame with `stats` or this call has returned it as SRF_ERR_TIMEOUT /
+   SRF_ERR_CAPACITY / SRF_ERR_STATE, which also clears it.  The layer operators (srf_grouped_matmul and its neighbours)
+   have a word of their own that this call alone returns, as SRF_ERR_TIMEOUT (2) or SRF_ERR_ARG (16), and clears; where
+   both are set, the first call returns the frames' error and the next one the layers'.  Synchronises
+   `stream`.  `flags` (may be NULL) receives both raw words, or-ed. */
 srf_status srf_check_errors(srf_ctx* ctx, void* stream, uint32_t* flags);
 
 /* Upper bound of live samples the context keeps scratch for; a frame with more samples is

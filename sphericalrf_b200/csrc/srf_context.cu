@@ -363,8 +363,16 @@ srf_status report_error_flags(srf_ctx* ctx, uint32_t flags, cudaStream_t s) {
     if (flags & 2u) return fail(ctx, SRF_ERR_TIMEOUT, "a wait on the tensor-core commit barrier expired");
     if (flags & 4u) return fail(ctx, SRF_ERR_CAPACITY, "the sample pool ran out of chunks");
     if (flags & 8u) return fail(ctx, SRF_ERR_STATE, "the fused grid refresh met a masked cell (the grid was changed behind the context)");
-    if (flags & 16u) return fail(ctx, SRF_ERR_ARG, "group offsets run backwards or point behind n_rows");
     return fail(ctx, SRF_ERR_CUDA, "unknown device error flag");
+}
+
+// The same for the word of the layer operators, which srf_check_errors alone reports: a frame must not fail for a layer call.
+srf_status report_layer_flags(srf_ctx* ctx, uint32_t flags, cudaStream_t s) {
+    if (!flags) return SRF_OK;
+    cudaMemsetAsync(&ctx->d_counters->layer_flags, 0, sizeof(unsigned int), s);
+    if (flags & 2u) return fail(ctx, SRF_ERR_TIMEOUT, "a layer call's wait for its loads or matrix instructions expired");
+    if (flags & 16u) return fail(ctx, SRF_ERR_ARG, "group offsets run backwards or point behind n_rows");
+    return fail(ctx, SRF_ERR_CUDA, "unknown device error flag of a layer call");
 }
 
 // Reads the error word back (synchronises `s`) and reports it.
@@ -1010,7 +1018,7 @@ srf_status srf_grouped_matmul(srf_ctx* ctx, const srf_grouped_t* in, const uint6
     const std::string why = refuse_matmul(in, d_offsets, d_x, d_w, d_y, &p);
     if (!why.empty()) return fail(ctx, SRF_ERR_ARG, why);
     DeviceGuard guard(ctx->device);
-    return launched(ctx, launch_grouped_matmul(p, d_offsets, d_x, d_w, d_y, &ctx->d_counters->error_flags, (cudaStream_t)stream));
+    return launched(ctx, launch_grouped_matmul(p, d_offsets, d_x, d_w, d_y, &ctx->d_counters->layer_flags, (cudaStream_t)stream));
 }
 
 srf_status srf_grouped_input_grad(srf_ctx* ctx, const srf_grouped_t* in, const uint64_t* d_offsets, const void* d_dy, const void* d_w,
@@ -1020,7 +1028,7 @@ srf_status srf_grouped_input_grad(srf_ctx* ctx, const srf_grouped_t* in, const u
     const std::string why = refuse_input_grad(in, d_offsets, d_dy, d_w, d_gate, d_dx, &p);
     if (!why.empty()) return fail(ctx, SRF_ERR_ARG, why);
     DeviceGuard guard(ctx->device);
-    return launched(ctx, launch_grouped_input_grad(p, d_offsets, d_dy, d_w, d_gate, d_dx, &ctx->d_counters->error_flags, (cudaStream_t)stream));
+    return launched(ctx, launch_grouped_input_grad(p, d_offsets, d_dy, d_w, d_gate, d_dx, &ctx->d_counters->layer_flags, (cudaStream_t)stream));
 }
 
 srf_status srf_grouped_weight_grad_workspace(srf_ctx* ctx, const srf_grouped_t* in, size_t* bytes) {
@@ -1042,7 +1050,7 @@ srf_status srf_grouped_weight_grad(srf_ctx* ctx, const srf_grouped_t* in, const 
     DeviceGuard guard(ctx->device);
     if (workspace_bytes < grouped_weight_grad_workspace(p, sm_count()))
         return fail(ctx, SRF_ERR_CAPACITY, "d_workspace is smaller than srf_grouped_weight_grad_workspace says");
-    return launched(ctx, launch_grouped_weight_grad(p, d_offsets, d_dy, d_x, d_dw, d_workspace, &ctx->d_counters->error_flags, (cudaStream_t)stream));
+    return launched(ctx, launch_grouped_weight_grad(p, d_offsets, d_dy, d_x, d_dw, d_workspace, &ctx->d_counters->layer_flags, (cudaStream_t)stream));
 }
 
 srf_status srf_grouped_matmul_fp8(srf_ctx* ctx, const srf_grouped_t* in, const uint64_t* d_offsets, const void* d_x, const float* d_x_scales,
@@ -1052,7 +1060,7 @@ srf_status srf_grouped_matmul_fp8(srf_ctx* ctx, const srf_grouped_t* in, const u
     const std::string why = refuse_matmul_fp8(in, d_offsets, d_x, d_x_scales, d_w, d_w_scales, d_y, &p);
     if (!why.empty()) return fail(ctx, SRF_ERR_ARG, why);
     DeviceGuard guard(ctx->device);
-    return launched(ctx, launch_grouped_matmul_fp8(p, d_offsets, d_x, d_x_scales, d_w, d_w_scales, d_y, &ctx->d_counters->error_flags, (cudaStream_t)stream));
+    return launched(ctx, launch_grouped_matmul_fp8(p, d_offsets, d_x, d_x_scales, d_w, d_w_scales, d_y, &ctx->d_counters->layer_flags, (cudaStream_t)stream));
 }
 
 srf_status srf_quantize_rows(srf_ctx* ctx, int type, uint64_t n_rows, const uint64_t* d_n_rows_used, uint32_t n_cols, const void* d_in,
@@ -1508,7 +1516,12 @@ srf_status srf_dump_samples(srf_ctx* ctx, const srf_view_t* view, uint64_t ray_f
 srf_status srf_check_errors(srf_ctx* ctx, void* stream, uint32_t* flags) {
     if (!ctx) return SRF_ERR_ARG;
     DeviceGuard guard(ctx->device);
-    return check_error_flags(ctx, (cudaStream_t)stream, flags);
+    const cudaStream_t s = (cudaStream_t)stream;
+    SRF_CK(ctx, cudaMemcpyAsync(&ctx->h_counters->layer_flags, &ctx->d_counters->layer_flags, sizeof(unsigned int), cudaMemcpyDeviceToHost, s));
+    const srf_status st = check_error_flags(ctx, s, flags);                  // synchronises
+    const uint32_t layer_flags = ctx->h_counters->layer_flags;
+    if (flags && st != SRF_ERR_CUDA) *flags |= layer_flags;
+    return st != SRF_OK ? st : report_layer_flags(ctx, layer_flags, s);      // behind a frame's error the layers' waits for the next call
 }
 
 srf_status srf_reserve(srf_ctx* ctx, uint64_t max_samples) {

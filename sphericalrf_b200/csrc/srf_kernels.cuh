@@ -29,8 +29,8 @@ struct NetMeta {
 // Device counters of one frame; zeroed before the count kernel.
 struct FrameCounters {
     unsigned long long n_alive, n_march_steps, n_samples, n_composited, n_hit;
-    unsigned int error_flags;
-    unsigned int pad;
+    unsigned int error_flags;      // of frames and stages
+    unsigned int layer_flags;      // of the layer operators: a frame does not fail for what a layer call met
 };
 
 // Per-ray record written by the count pass.

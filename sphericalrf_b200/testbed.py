@@ -101,7 +101,7 @@ class Renderer:
         self._ck(self.lib.srf_reserve(self.ctx, max_samples))
 
     def check_errors(self, stream=None):
-        """srf_check_errors: raises if a frame enqueued since the last check was cut short on the device."""
+        """srf_check_errors: raises if a frame enqueued since the last check was cut short on the device, or a layer call met bad offsets."""
         self._ck(self.lib.srf_check_errors(self.ctx, stream, None))
 
     def set_timing(self, on=True):

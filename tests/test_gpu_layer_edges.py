@@ -2,7 +2,8 @@
 import pytest
 
 from sphericalrf_b200 import abi
-from test_gpu_layers import POISON, TYPES, Case8, check_rows, r, table, up  # noqa: F401  (r is the fixture)
+from helpers import make_renderer, small_scene
+from test_gpu_layers import POISON, TYPES, Case, Case8, check_rows, r, table, up  # noqa: F401  (r is the fixture)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -65,3 +66,24 @@ def test_scales_that_are_not_finite_stay_in_their_rows(r, bad):  # noqa: F811
     rest = torch.arange(100, device="cuda") != 40
     exact, terms = c.exact()
     assert bool(((y.double() - exact).abs() <= 1.001 * 262 * 2.0 ** -23 * terms)[rest].all())
+
+
+def test_frames_do_not_fail_for_a_layer_call(built_lib):
+    """Bad offsets of a layer call are the layer's error: frames in between render, srf_check_errors reports them once."""
+    sc = small_scene()
+    ren = make_renderer(sc)
+    post = abi.default_post()
+    want = ren.render(sc["view"], post)
+    c = Case([30, 30, 40], 64, 64, "f16", 9)
+    y = torch.zeros(c.n_rows, 64, dtype=torch.float16, device="cuda")
+    ren.grouped_matmul_device(c.layer(abi.TYPE_F16), torch.tensor([0, 50, 40, 100], device="cuda"), c.x, c.w, y)
+    torch.cuda.synchronize()
+    assert (ren.render(sc["view"], post) == want).all()
+    frame = ren.render_frame(sc["view"], post, want_stats=True)
+    assert frame["stats"]["error_flags"] == 0
+    ren.dump_samples(sc["view"], 0, 10, 1 << 20)
+    with pytest.raises(abi.SrfError, match="offsets") as e:
+        ren.check_errors()
+    assert e.value.status == abi.ERR_ARG
+    ren.check_errors()
+    ren.close()
