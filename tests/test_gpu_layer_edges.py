@@ -3,7 +3,7 @@ import pytest
 
 from sphericalrf_b200 import abi
 from helpers import make_renderer, small_scene
-from test_gpu_layers import POISON, TYPES, Case, Case8, check_rows, r, table, up  # noqa: F401  (r is the fixture)
+from test_gpu_layers import POISON, TYPES, Case, Case8, Chain, check_rows, r, table, up  # noqa: F401  (r is the fixture)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -87,3 +87,30 @@ def test_frames_do_not_fail_for_a_layer_call(built_lib):
     assert e.value.status == abi.ERR_ARG
     ren.check_errors()
     ren.close()
+
+
+def test_calls_without_a_stream_run_on_the_current_one(r):  # noqa: F811
+    """Behind torch's work on a stream of its own, and captured with it."""
+    c = Chain(r, [500, 20, 0, 4000], 1)
+    c.step()
+    want = c.results()
+    c.clear()
+    torch.cuda.synchronize()
+    s, x = torch.cuda.Stream(), c.h[0].clone()
+    c.h[0].zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(20_000_000)          # the samples arrive late
+        c.h[0].copy_(x)
+        c.step()
+        got = [t.clone() for t in c.h[1:] + c.d[:3] + c.dw]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    c.clear()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.step()
+    assert all(bool((t == 0).all()) for t in c.results())
+    g.replay()
+    assert all(torch.equal(a, b) for a, b in zip(c.results(), want))
