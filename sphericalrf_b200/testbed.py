@@ -30,6 +30,51 @@ def _stream(device, stream):
     return torch._C._cuda_getCurrentRawStream(device)      # torch.cuda.current_stream(device).cuda_stream takes 1.2 us, this 0.06
 
 
+_DTYPES = {}       # value type of the layer operators -> torch's type
+
+
+def _dtypes():
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({abi.TYPE_F16: torch.float16, abi.TYPE_BF16: torch.bfloat16, abi.TYPE_F32: torch.float32,
+                        abi.TYPE_E4M3: torch.float8_e4m3fn, "index": torch.int64})
+    return _DTYPES
+
+
+def _reach(t):
+    """Values from the tensor's first one to the end of its memory."""
+    return t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+
+
+def _same(kind, dtype):
+    """Types that hold the same bits."""
+    import torch
+    return (kind, dtype) in ((torch.float8_e4m3fn, torch.uint8), (torch.int64, torch.uint64))
+
+
+def _tensors(device, *wanted):
+    """Refuses tensors that a call would misread or leave: (name, tensor or None, type, values) each.  The tensors'
+    properties take 2 us of the 9 that a small call takes through Python; a captured call pays nothing."""
+    for name, t, kind, count in wanted:
+        if t is None or kind is None or count < 1:        # not given, of a type that the library refuses, or not used
+            continue
+        if t.dtype is not kind and not _same(kind, t.dtype):
+            raise abi.SrfError(abi.ERR_ARG, f"{name} is of type {t.dtype}, the call needs {kind}")
+        if t.get_device() != device:
+            raise abi.SrfError(abi.ERR_ARG, f"{name} is on {t.device}, the context on cuda:{device}")
+        if (t.numel() < count or not t.is_contiguous()) and _reach(t) < count:
+            raise abi.SrfError(abi.ERR_ARG, f"{name} has memory for {_reach(t)} values, the call needs {count}")
+
+
+def _values(layer):
+    """Values from the first to behind the last one of n_in-wide samples, n_out-wide samples and the matrices."""
+    n, n_in, n_out, more = layer.n_rows - 1, layer.n_in, layer.n_out, layer.n_groups - 1
+    ld_w = layer.ld_w or n_in
+    matrix = (n_out - 1) * ld_w + n_in
+    return (n * (layer.ld_x or n_in) + n_in, n * (layer.ld_y or n_out) + n_out,
+            matrix + more * (layer.group_stride or n_out * ld_w) if more else matrix)
+
+
 class Renderer:
     """One library context on one GPU."""
 
@@ -253,13 +298,23 @@ class Renderer:
                     dloss=dl.cpu().numpy(), loss=loss.cpu().numpy(), reg=reg.cpu().numpy())
 
     # -- layers of fields cut into regions: torch CUDA tensors in and out, enqueued on `stream` (a raw cudaStream_t; None: torch's
-    #    current stream of the context's device, on which the tensors' own work runs) --
+    #    current stream of the context's device, on which the tensors' own work runs).  Tensors of another type, on another
+    #    device or with less memory than the call describes are refused; strides are the call's, as in C --
     def grouped_matmul_device(self, layer, offsets, x, w, y, stream=None):
         """srf_grouped_matmul: y[r] = act(W[g] x[r]); `layer` from abi.make_grouped, `offsets` (n_groups + 1,) int64 or None."""
-        self._ck(self.lib.srf_grouped_matmul(self.ctx, layer, _dev_ptr(offsets), x.data_ptr(), w.data_ptr(), y.data_ptr(), _stream(self.device, stream)))
+        d, (n_x, n_y, n_w) = _DTYPES or _dtypes(), _values(layer)
+        t = d.get(layer.type)
+        _tensors(self.device, ("offsets", offsets, d["index"], layer.n_groups + 1), ("x", x, t, n_x), ("w", w, t, n_w),
+                 ("y", y, d.get(layer.out_type), n_y))
+        self._ck(self.lib.srf_grouped_matmul(self.ctx, layer, _dev_ptr(offsets), x.data_ptr(), w.data_ptr(), y.data_ptr(),
+                                             _stream(self.device, stream)))
 
     def grouped_input_grad_device(self, layer, offsets, dy, w, gate, dx, stream=None):
         """srf_grouped_input_grad: dx[r] = W[g]^T dy[r], 0 where `gate` (or None) is not > 0."""
+        d, (n_x, n_y, n_w) = _DTYPES or _dtypes(), _values(layer)
+        t = d.get(layer.type)
+        _tensors(self.device, ("offsets", offsets, d["index"], layer.n_groups + 1), ("dy", dy, t, n_y), ("w", w, t, n_w),
+                 ("gate", gate, t, n_x), ("dx", dx, d.get(layer.out_type), n_x))
         self._ck(self.lib.srf_grouped_input_grad(self.ctx, layer, _dev_ptr(offsets), dy.data_ptr(), w.data_ptr(), _dev_ptr(gate),
                                                  dx.data_ptr(), _stream(self.device, stream)))
 
@@ -271,21 +326,39 @@ class Renderer:
 
     def grouped_weight_grad_device(self, layer, offsets, dy, x, dw, workspace, stream=None):
         """srf_grouped_weight_grad: dW[g] = sum over the group's samples of dy[r] x[r]^T."""
+        d, (n_x, n_y, n_w) = _DTYPES or _dtypes(), _values(layer)
+        t = d.get(layer.type)
+        _tensors(self.device, ("offsets", offsets, d["index"], layer.n_groups + 1), ("dy", dy, t, n_y), ("x", x, t, n_x),
+                 ("dw", dw, d.get(layer.out_type), n_w), ("workspace", workspace, workspace.dtype, workspace.numel()))
         self._ck(self.lib.srf_grouped_weight_grad(self.ctx, layer, _dev_ptr(offsets), dy.data_ptr(), x.data_ptr(), dw.data_ptr(),
-                                                  workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(self.device, stream)))
+                                                  workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                                                  _stream(self.device, stream)))
 
     def grouped_matmul_fp8_device(self, layer, offsets, x, x_scales, w, w_scales, y, stream=None):
         """srf_grouped_matmul_fp8: the layer on e4m3 values and block scales (quantize_rows_device, quantize_weights_device)."""
+        d, (n_x, n_y, n_w), groups, kb = _DTYPES or _dtypes(), _values(layer), layer.n_groups, (layer.n_in + 127) // 128
+        t, f32 = d.get(layer.type), d[abi.TYPE_F32]
+        _tensors(self.device, ("offsets", offsets, d["index"], groups + 1), ("x", x, t, n_x), ("x_scales", x_scales, f32, kb * layer.n_rows),
+                 ("w", w, t, n_w), ("w_scales", w_scales, f32, groups * kb * ((layer.n_out + 127) // 128)),
+                 ("y", y, d.get(layer.out_type), n_y))
         self._ck(self.lib.srf_grouped_matmul_fp8(self.ctx, layer, _dev_ptr(offsets), x.data_ptr(), x_scales.data_ptr(), w.data_ptr(),
                                                  w_scales.data_ptr(), y.data_ptr(), _stream(self.device, stream)))
 
     def quantize_rows_device(self, type, n_rows, n_cols, values, ld_in, out, ld_out, scales, n_rows_used=None, stream=None):
         """srf_quantize_rows: one scale per row and 128 columns; `scales` (ceil(n_cols / 128), n_rows)."""
+        d = _DTYPES or _dtypes()
+        _tensors(self.device, ("values", values, d.get(type), (n_rows - 1) * (ld_in or n_cols) + n_cols),
+                 ("out", out, d[abi.TYPE_E4M3], (n_rows - 1) * (ld_out or n_cols) + n_cols),
+                 ("scales", scales, d[abi.TYPE_F32], (n_cols + 127) // 128 * n_rows), ("n_rows_used", n_rows_used, d["index"], 1))
         self._ck(self.lib.srf_quantize_rows(self.ctx, type, n_rows, _dev_ptr(n_rows_used), n_cols, values.data_ptr(), ld_in,
                                             out.data_ptr(), ld_out, scales.data_ptr(), _stream(self.device, stream)))
 
     def quantize_weights_device(self, type, n_matrices, n_rows, n_cols, values, ld_in, out, ld_out, scales, stream=None):
         """srf_quantize_weights: one scale per 128 x 128 block."""
+        d, rows = _DTYPES or _dtypes(), n_matrices * n_rows
+        _tensors(self.device, ("values", values, d.get(type), (rows - 1) * (ld_in or n_cols) + n_cols),
+                 ("out", out, d[abi.TYPE_E4M3], (rows - 1) * (ld_out or n_cols) + n_cols),
+                 ("scales", scales, d[abi.TYPE_F32], n_matrices * ((n_rows + 127) // 128) * ((n_cols + 127) // 128)))
         self._ck(self.lib.srf_quantize_weights(self.ctx, type, n_matrices, n_rows, n_cols, values.data_ptr(), ld_in, out.data_ptr(),
                                                ld_out, scales.data_ptr(), _stream(self.device, stream)))
 
