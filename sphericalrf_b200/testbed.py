@@ -62,8 +62,11 @@ def _tensors(device, *wanted):
             raise abi.SrfError(abi.ERR_ARG, f"{name} is of type {t.dtype}, the call needs {kind}")
         if t.get_device() != device:
             raise abi.SrfError(abi.ERR_ARG, f"{name} is on {t.device}, the context on cuda:{device}")
-        if (t.numel() < count or not t.is_contiguous()) and _reach(t) < count:
-            raise abi.SrfError(abi.ERR_ARG, f"{name} has memory for {_reach(t)} values, the call needs {count}")
+        if t.numel() < count or not t.is_contiguous():
+            if _reach(t) < count:
+                raise abi.SrfError(abi.ERR_ARG, f"{name} has memory for {_reach(t)} values, the call needs {count}")
+            if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:     # a transposed view: rows with gaps have their values side by side
+                raise abi.SrfError(abi.ERR_ARG, f"{name} has values of a row {t.stride(-1)} apart")
 
 
 def _values(layer):

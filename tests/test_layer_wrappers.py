@@ -133,3 +133,10 @@ def test_padded_rows_and_nothing_are_taken(rec):
     assert len(rec.lib.calls) == 3
     with pytest.raises(abi.SrfError, match="x has memory for 639"):
         rec.grouped_matmul_device(layer, None, torch.zeros(639, dtype=torch.float16), w, y, stream=0)
+
+
+@pytest.mark.parametrize("name", ["x", "y", "w", "gate", "dw", "x8", "w8", "ws"])
+def test_transposed_views_are_refused(rec, name):
+    t = tensors()[name]
+    wide = torch.zeros(4, 4, t.numel(), dtype=torch.uint8).to(t.dtype)       # memory enough for every stride
+    refused(rec, {name: wide[:, :, :t.numel() // 2].transpose(1, 2)}, name, "values of a row")
