@@ -1001,10 +1001,13 @@ srf_status srf_network_density(srf_ctx* ctx, const float* d_positions, uint64_t 
 
 namespace {
 
+// The launch wrappers look at every return code: `why` is all there is to know, and an error that the host program left on the
+// thread is not ours (a call without samples launches nothing, and would report it).  A failed launch leaves its own error
+// there, which is taken off: the next one to ask would take it for theirs.
 srf_status launched(srf_ctx* ctx, const char* why) {
-    if (why) return fail(ctx, SRF_ERR_CUDA, why);
-    SRF_CK(ctx, cudaGetLastError());
-    return SRF_OK;
+    if (!why) return SRF_OK;
+    const cudaError_t e = cudaGetLastError();
+    return fail(ctx, SRF_ERR_CUDA, e == cudaSuccess ? std::string(why) : std::string(why) + ": " + cudaGetErrorString(e));
 }
 
 }  // namespace

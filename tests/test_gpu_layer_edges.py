@@ -1,4 +1,6 @@
 """Edges of the layer operators beside those of test_gpu_layers.py, whose bounds and cases these tests use."""
+import ctypes as C
+
 import pytest
 
 from sphericalrf_b200 import abi
@@ -114,3 +116,54 @@ def test_calls_without_a_stream_run_on_the_current_one(r):  # noqa: F811
     assert all(bool((t == 0).all()) for t in c.results())
     g.replay()
     assert all(torch.equal(a, b) for a, b in zip(c.results(), want))
+
+
+@pytest.fixture
+def cudart(r):  # noqa: F811
+    """The CUDA runtime that torch and the library share."""
+    lib = C.CDLL("libcudart.so.12")
+    lib.cudaStreamBeginCapture.argtypes = [C.c_void_p, C.c_int]
+    lib.cudaStreamSynchronize.argtypes = [C.c_void_p]
+    lib.cudaStreamEndCapture.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
+    assert lib.cudaGetLastError() == 0
+    yield lib
+    lib.cudaGetLastError()
+
+
+def test_an_older_error_of_the_thread_is_not_the_calls(r, cudart):  # noqa: F811
+    """A launch that succeeds takes an older error off the thread; a call without samples launches nothing."""
+    none, w = torch.zeros(0, dtype=torch.float16, device="cuda"), torch.zeros(1, 64, 64, dtype=torch.float16, device="cuda")
+    layer, stream = abi.make_grouped(1, 0, 64, 64), torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    try:
+        assert cudart.cudaSetDevice(4096) != 0                 # the host program's own mistake
+        left = cudart.cudaPeekAtLastError()
+        assert left != 0
+        r.grouped_matmul_device(layer, None, none, w, none, stream)
+        r.grouped_input_grad_device(layer, None, none, w, None, none, stream)
+        r.quantize_rows_device(abi.TYPE_F16, 0, 64, none, 64, none, 64, none, stream=stream)
+        assert cudart.cudaPeekAtLastError() == left            # still there for the host program to see
+    finally:
+        cudart.cudaGetLastError()
+
+
+def test_a_failed_launch_leaves_no_error_behind(r, cudart):  # noqa: F811
+    """A launch into a capture that a synchronisation has broken is refused by the runtime."""
+    c = Case([300], 64, 48, "f16", 8)
+    y = torch.full((300, 48), POISON, dtype=torch.float16, device="cuda")
+    layer, s, graph = c.layer(abi.TYPE_F16), torch.cuda.Stream(), C.c_void_p()
+    torch.cuda.synchronize()
+    try:
+        assert cudart.cudaStreamBeginCapture(s.cuda_stream, 0) == 0
+        assert cudart.cudaStreamSynchronize(s.cuda_stream) != 0
+        cudart.cudaGetLastError()
+        with pytest.raises(abi.SrfError, match="did not launch: ") as e:
+            r.grouped_matmul_device(layer, c.offsets, c.x, c.w, y, s.cuda_stream)
+        assert e.value.status == abi.ERR_CUDA
+        assert cudart.cudaPeekAtLastError() == 0
+    finally:
+        cudart.cudaStreamEndCapture(s.cuda_stream, C.byref(graph))       # reports the broken capture
+        cudart.cudaGetLastError()
+    r.grouped_matmul_device(layer, c.offsets, c.x, c.w, y)
+    torch.cuda.synchronize()
+    assert not bool((y == POISON).any())
