@@ -97,22 +97,25 @@ __device__ __forceinline__ uint2 to_e4m3(const float (&q)[8]) {
     return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
 }
 
-// The short way, two values to an instruction.
+// The short way, two values to an instruction.  It makes the negative of the quotient, -q0 - r (v - q0 s), and turns the sign of
+// the result: where q0 is exact the remainder is +0, which leaves the sign of -q0 = -0 or +0 alone (added to q0 = -0, it would
+// make it +0).
 __device__ __forceinline__ uint2 quantize8_plain(const float (&f)[8], float scale, float inverse) {
-    uint64_t down, inv;
-    asm("mov.b64 %0, {%1, %1};" : "=l"(down) : "f"(-scale));
-    asm("mov.b64 %0, {%1, %1};" : "=l"(inv) : "f"(inverse));
+    uint64_t up, inv;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(up) : "f"(scale));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(inv) : "f"(-inverse));
     float q[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         uint64_t v, q0, rest;
         asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(f[2 * i]), "f"(f[2 * i + 1]));
         asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q0) : "l"(v), "l"(inv));
-        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(rest) : "l"(q0), "l"(down), "l"(v));
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(rest) : "l"(q0), "l"(up), "l"(v));
         asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(q0) : "l"(rest), "l"(inv));
         asm("mov.b64 {%0, %1}, %2;" : "=f"(q[2 * i]), "=f"(q[2 * i + 1]) : "l"(q0));
     }
-    return to_e4m3(q);
+    const uint2 n = to_e4m3(q);
+    return make_uint2(n.x ^ 0x80808080u, n.y ^ 0x80808080u);
 }
 
 __device__ __forceinline__ uint2 quantize8(const float (&f)[8], const BlockScale& b) {

@@ -1,11 +1,12 @@
 """Edges of the layer operators beside those of test_gpu_layers.py, whose bounds and cases these tests use."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
 from sphericalrf_b200 import abi
 from helpers import make_renderer, small_scene
-from test_gpu_layers import POISON, TYPES, Case, Case8, Chain, check_rows, r, table, up  # noqa: F401  (r is the fixture)
+from test_gpu_layers import POISON, TYPES, Case, Case8, Chain, check_rows, e4m3_reference, r, scale_reference, table, up  # noqa: F401  (r is the fixture)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -167,3 +168,36 @@ def test_a_failed_launch_leaves_no_error_behind(r, cudart):  # noqa: F811
     r.grouped_matmul_device(layer, c.offsets, c.x, c.w, y)
     torch.cuda.synchronize()
     assert not bool((y == POISON).any())
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(64, 512), (37, 200)])
+@pytest.mark.parametrize("what", ["plain", "tiny", "nan"])
+def test_quantised_zeros_keep_their_sign(r, what, rows, cols, kind):  # noqa: F811
+    """Whichever way a block's quotients are taken: all values ordinary, a tiny scale, a NaN beside them."""
+    type_id, dt = TYPES[kind]
+    gen = torch.Generator().manual_seed(rows)
+    v = torch.randn(rows, cols, generator=gen)
+    v[torch.rand(rows, cols, generator=gen) < 0.3] = -0.0
+    v[torch.rand(rows, cols, generator=gen) < 0.3] = 0.0
+    v[0, :128] = -0.0                                     # a block of negative zeros
+    v = (v * (2.0 ** -110 if what == "tiny" and kind == "bf16" else 1.0)).to(dt)
+    if what == "nan":
+        v[::5, 3] = float("nan")
+    dev = v.cuda()
+    for per in (1, 128):
+        q = torch.full((rows, up(cols, 16)), 0x55, dtype=torch.uint8, device="cuda")
+        nb, nr = up(cols, 128) // 128, up(rows, 128) // 128
+        if per == 1:
+            scales = torch.zeros(nb, rows, device="cuda")
+            r.quantize_rows_device(type_id, rows, cols, dev, cols, q, q.stride(0), scales)
+        else:
+            scales = torch.zeros(1, nr, nb, device="cuda")
+            r.quantize_weights_device(type_id, 1, rows, cols, dev, cols, q, q.stride(0), scales)
+        torch.cuda.synchronize()
+        f, want = v.float().numpy(), np.full(q.shape, 0x55, np.uint8)
+        for i in range(0, rows, per):
+            for j in range(0, cols, 128):
+                block = f[i:i + per, j:min(cols, j + 128)]
+                want[i:i + per, j:min(cols, j + 128)] = e4m3_reference(block, scale_reference(block))
+        assert np.array_equal(q.cpu().numpy(), want), f"rows {per}"
