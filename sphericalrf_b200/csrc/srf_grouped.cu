@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_weight_grad_join(const Grouped
             constexpr size_t kSlot = (size_t)CG * kBM * BN / 4;
 #pragma unroll 4
             for (uint32_t v = v0 + part; v <= v1; v += LANES) {
-                const float4 e = q[(2 * (size_t)v + (v == v0 ? 1 : 0)) * kSlot];
+                const float4 e = __ldcg(q + (2 * (size_t)v + (v == v0 ? 1 : 0)) * kSlot);
                 sum.x += e.x; sum.y += e.y; sum.z += e.z; sum.w += e.w;
             }
         }

@@ -52,7 +52,9 @@ template <int BN, int CG> __host__ __device__ constexpr int smem_bytes() {
     return b < kSmemMin ? kSmemMin : b;
 }
 
-// Copies of one lane's own values into shared memory, in groups that complete in order.
+// Copies of one lane's own values into shared memory, in groups that complete in order.  Copies of 4 bytes exist through L1 only;
+// they are ordinary loads for memory order, so the wait for the kernel in front (a quantisation that writes the scales)
+// orders them.
 __device__ __forceinline__ void copy_async4(float* dst, const float* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(smem_u32(dst)), "l"(src) : "memory");
 }

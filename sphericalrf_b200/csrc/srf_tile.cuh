@@ -64,8 +64,9 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // Programmatic dependent launch: a kernel's blocks may be set up while the kernel in front of it in the stream still runs.
-// Nothing in global memory is touched in front of wait_for_inputs(), which returns when that kernel has completed.  Loads
-// behind it go to L2 (__ldcg) or through TMA, never the read-only path: that may keep lines from the time before.
+// Nothing in global memory is touched in front of wait_for_inputs(), which returns when that kernel has completed and its
+// writes are visible.  Loads behind it are ordinary ones (through L2 where nothing is read twice) or TMA's, never the
+// read-only path: the data was not read-only while this kernel was on the GPU.
 __device__ __forceinline__ void wait_for_inputs() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

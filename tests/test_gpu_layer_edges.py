@@ -201,3 +201,35 @@ def test_quantised_zeros_keep_their_sign(r, what, rows, cols, kind):  # noqa: F8
                 block = f[i:i + per, j:min(cols, j + 128)]
                 want[i:i + per, j:min(cols, j + 128)] = e4m3_reference(block, scale_reference(block))
         assert np.array_equal(q.cpu().numpy(), want), f"rows {per}"
+
+
+def test_8_bit_calls_see_each_other(r):  # noqa: F811
+    """Samples and weights to 8 bits and the layer on them, over and over in the same buffers: without waits the bits of the
+    same chain with a wait after every step.  Scales change by powers of two from turn to turn."""
+    n, k, off = 3000, 256, torch.tensor([0, 1200, 1200, 3000], device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    start = torch.randn(n, k, generator=gen, device="cuda").half()
+    w0 = (torch.randn(3, k, k, generator=gen, device="cuda") / 16).half()
+    layer = abi.make_grouped(3, n, k, k, abi.TYPE_E4M3, abi.TYPE_F16)
+
+    def chain(wait):
+        h, w, y = start.clone(), w0.clone(), torch.zeros(n, k, dtype=torch.float16, device="cuda")
+        q, qs = torch.zeros(n, k, dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros(k // 128, n, device="cuda")
+        w8, ws = torch.zeros(3, k, k, dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros(3, k // 128, k // 128, device="cuda")
+        seen = []
+        for i in range(30):
+            r.quantize_weights_device(abi.TYPE_F16, 3, k, k, w, k, w8, k, ws)
+            wait()
+            r.quantize_rows_device(abi.TYPE_F16, n, k, h, k, q, k, qs)
+            wait()
+            r.grouped_matmul_fp8_device(layer, off, q, qs, w8, ws, y)
+            wait()
+            seen.append(y.clone())
+            h.copy_(y).clamp_(-8, 8).add_(start, alpha=2.0 ** (i % 5 - 2))
+            w.copy_(w0).mul_(2.0 ** (i % 3))
+            wait()
+        torch.cuda.synchronize()
+        return seen + [q.view(torch.uint8), qs, w8.view(torch.uint8), ws]
+
+    for got, want in zip(chain(lambda: None), chain(torch.cuda.synchronize)):
+        assert torch.equal(got, want)
