@@ -333,8 +333,13 @@ srf_status srf_volume_rendering_loss(srf_ctx* ctx, const srf_loss_params_t* para
        backwards or point behind n_rows are cut to the buffer and reported by srf_check_errors as SRF_ERR_ARG; the
        call's output is then meaningless (n_rows = 0 launches no product and reports nothing).  d_offsets NULL: one
        group of all n_rows rows (n_groups = 1);
-     - products are summed in fp32 and rounded once to out_type; no call allocates, synchronises or keeps state, so all
-       of them can be captured, and calls on different streams may overlap. */
+     - products are summed in fp32 and rounded once to out_type.  The tensor core's own additions truncate; results in
+       fp32, and in fp16 behind 8192 products, are sums of runs of 512 products added with rounding: 2.8e-6 of the sum at
+       most where all products have one sign, 2-norm 7e-7 where they have not (8e-7 at 2^20 products, growing with the
+       square root of their number).  Other 16-bit results are off by at most a ninth of the half step of their rounding
+       before it (5.3e-5 of a sum of 8192 products of one sign, 4.3e-4 of one of 65536 in bf16);
+     - no call allocates, synchronises or keeps state, so all of them can be captured, and calls on different streams may
+       overlap. */
 typedef struct srf_grouped_t {
     uint32_t struct_size;        /* sizeof(srf_grouped_t), checked */
     uint32_t n_groups;           /* 1 .. 4096 */

@@ -18,10 +18,13 @@
 // are 160 to 256 columns wide, in steps of 32, so that the columns divide evenly: 656 columns are three tiles of 224 (66
 // groups of 1057 samples, 780 -> 656: 84.7 us against 88.7).
 //
-// The tensor core's additions to an accumulator truncate, so that a long sum's error grows with its length (2-norm 2.1e-6 at
-// 2048 products, 9e-6 at 8192, where fp32 additions one by one have 4e-7): nothing beside a rounding to 16 bits, but not
-// what a result in fp32 should have.  LONG kernels therefore start a new accumulator every 512 products and add those in
-// registers, rounded (5e-7 at any length); both sets of epilogue warps work on every tile then, half of its columns each.
+// The tensor core's additions to an accumulator truncate, so that a long sum's error grows with its length: 2-norm 2.5e-6 at 2048
+// products of mixed signs, 9.7e-6 at 8192, 7.7e-5 at 65536; sums of one sign fall short by 1.3e-5, 5.3e-5 and 4.3e-4 of themselves.
+// That is little beside a rounding to bf16, or to fp16 up to 8192 products, but not what a result in fp32 should have.  LONG
+// kernels therefore start a new accumulator every 512 products (6.4e-7; 2.8e-6 for one sign) and add those in registers, rounded;
+// both sets of epilogue warps work on every tile then, half of its columns each.  The rounded additions of m such runs, one by one,
+// have an error of their own that grows with sqrt(m): weight gradients have 4.8e-7 at 2^14 samples, 5.8e-7 at 2^18, 8.4e-7 at 2^20
+// where one worker owns a whole sum (shorter where the sum is cut), and some 4e-6 at 2^24.
 //
 // Measured (one B200): 32801 samples in 16 groups, 2048 -> 2043: 179 us alone (1.53 PFLOP/s, tensor pipe 93 %), 214-222 us a call
 // under the power limit (single CTAs 241); 160 samples in 64 groups, 2048 -> 1408: 63-67 us, 5.7 TB/s of matrices; 1048613
@@ -423,7 +426,7 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         store_rows(rs, stage);
                     }
                 }
-            } else if (MODE == kWeightGrad) {
+            } else {
                 constexpr int kPer = kCols < 64 ? kCols : 64;
 #pragma unroll
                 for (int c = 0; c < kCols; c += kPer) {
@@ -432,12 +435,22 @@ k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     for (int u = 0; u < kPer / 8; ++u) {
                         uint32_t w[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = pack16(lo_of(sum[c / 2 + 4 * u + e]), hi_of(sum[c / 2 + 4 * u + e]), rs.bf16);
+                        for (int e = 0; e < 4; ++e) {
+                            const float lo = lo_of(sum[c / 2 + 4 * u + e]), hi = hi_of(sum[c / 2 + 4 * u + e]);
+                            w[e] = MODE == kLayer && p.relu ? pack16_relu(lo, hi, rs.bf16) : pack16(lo, hi, rs.bf16);
+                        }
                         stage_unit(stage, lane, u, make_uint4(w[0], w[1], w[2], w[3]));
                     }
                     rs.bytes = (cols - c < (uint32_t)kPer ? cols - c : (uint32_t)kPer) * 2u;
                     rs.out = out + (size_t)c * 2;
-                    store_rows(rs, stage);
+                    if (MODE == kInputGrad && p.gate) {
+                        uint4 hv[8];
+                        rs.gate = p.gate + row0 * p.gate_row_bytes + (size_t)(col0 + c) * 2;
+                        load_gate(rs, hv);
+                        store_rows<true>(rs, stage, hv);
+                    } else {
+                        store_rows(rs, stage);
+                    }
                 }
             }
         }
@@ -666,6 +679,13 @@ WeightGradPlan plan_weight_grad(const srf_grouped_t& p, int sms) {
     return w;
 }
 
+// Whether sums of `depth` products take a LONG kernel.  One accumulator is off by up to 1.3e-5 of the sum at 2048 products of one
+// sign, 5.3e-5 at 8192, 4.3e-4 at 65536 (a LONG kernel 2.8e-6 at all of them): too much for an fp32 result; a ninth of fp16's half
+// step of 4.9e-4 at 8192, but all of it at 65536; at most a ninth of bf16's 3.9e-3 at any depth.
+bool long_sums(const srf_grouped_t& p, uint32_t depth) {
+    return p.out_type == SRF_TYPE_F32 ? depth > kChunk * kBK : p.out_type == SRF_TYPE_F16 && depth > 8192;
+}
+
 template <int MODE, int BN, int CG, bool LONG>
 const char* launch(const CUtensorMap& a, const CUtensorMap& b, const GroupedArgs& args, uint32_t grid, cudaStream_t stream) {
     static_assert(smem_bytes<BN, CG>() <= 227 * 1024, "shared memory of one SM");
@@ -748,7 +768,7 @@ const char* launch_grouped_matmul(const srf_grouped_t& p, const uint64_t* offset
                                   unsigned int* error_flags, cudaStream_t stream) {
     if (!p.n_rows) return nullptr;
     const int sms = sm_count();
-    const TileShape t = pick_tile(p, p.n_out, sms, p.out_type == SRF_TYPE_F32 && p.n_in > kChunk * kBK ? 64 : 32, 32);
+    const TileShape t = pick_tile(p, p.n_out, sms, long_sums(p, p.n_in) ? 64 : 32, 32);
     CUtensorMap a, b;
     if (!make_operand_map(&a, x, p.type, p.n_in, p.n_rows, p.ld_x, 0, 0, t.cg == 2 ? kBM : kRowBox) ||
         !make_operand_map(&b, w, p.type, p.n_in, p.n_out, p.ld_w, p.n_groups, p.group_stride, t.bn / t.cg))
@@ -759,7 +779,7 @@ const char* launch_grouped_matmul(const srf_grouped_t& p, const uint64_t* offset
     k.f32 = p.out_type == SRF_TYPE_F32; k.bf16 = p.type == SRF_TYPE_BF16; k.relu = p.activation == SRF_ACT_RELU;
     k.out_row_bytes = p.ld_y * (k.f32 ? 4 : 2); k.out_cols = p.n_out; k.depth = p.n_in; k.width = t.bn; k.error_flags = error_flags;
     const uint32_t grid = tile_grid(p, p.n_out, t, sms);
-    if (k.f32 && p.n_in > kChunk * kBK) return launch_long<kLayer>(a, b, k, t, grid, stream);
+    if (long_sums(p, p.n_in)) return launch_long<kLayer>(a, b, k, t, grid, stream);
     if (t.cg == 2) return launch<kLayer, 256, 2, false>(a, b, k, grid, stream);
     switch (t.bn) {
     case 256: return launch<kLayer, 256, 1, false>(a, b, k, grid, stream);
@@ -785,7 +805,7 @@ const char* launch_grouped_input_grad(const srf_grouped_t& p, const uint64_t* of
     k.out_row_bytes = p.ld_x * (k.f32 ? 4 : 2); k.gate_row_bytes = p.ld_x * 2; k.out_cols = p.n_in; k.depth = p.n_out; k.width = t.bn;
     k.error_flags = error_flags;
     const uint32_t grid = tile_grid(p, p.n_in, t, sms);
-    if (k.f32 && p.n_out > kChunk * kBK) return launch_long<kInputGrad>(a, b, k, t, grid, stream);
+    if (long_sums(p, p.n_out)) return launch_long<kInputGrad>(a, b, k, t, grid, stream);
     if (t.cg == 2) return launch<kInputGrad, 256, 2, false>(a, b, k, grid, stream);
     switch (t.bn) {
     case 256: return launch<kInputGrad, 256, 1, false>(a, b, k, grid, stream);

@@ -33,8 +33,8 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
                  : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done != 0;
 }
-// Longest wait on one barrier, in cycles (about four seconds).  The longest wait that real work causes is the
-// accumulation of one output tile over 2^26 rows, well under a second.
+// Longest wait on one barrier, in cycles (about four seconds).  The longest wait that real work causes is for one accumulator:
+// 1024 stages of a sum of 65536 products, well under a millisecond.
 constexpr long long kWaitCycles = 8000000000ll;
 
 // Bounded wait of one thread.  `failed` (shared memory) tells the CTA's other warps that one of them gave up.

@@ -233,3 +233,31 @@ def test_8_bit_calls_see_each_other(r):  # noqa: F811
 
     for got, want in zip(chain(lambda: None), chain(torch.cuda.synchronize)):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("sizes,n_in,n_out,relu", [
+    ([130, 0, 37], 65536, 40, True), ([3], 16500, 1, False), ([300, 60], 9001, 300, True), ([20000, 3, 20001], 8200, 300, False)])
+def test_deep_sums_are_rounded_once(r, sizes, n_in, n_out, relu):  # noqa: F811
+    """fp16 results of long sums of one sign, where an accumulator that truncates falls short of the sum by as much as the
+    rounding itself (4.3e-4 at 65536 products).  Sums are cut into runs of 512 like those of fp32 results: half a step of
+    fp16 and (512 + runs) 2^-23 of the sum, at most 7.7e-5."""
+    c = Case(sizes, n_in, n_out, "f16", 500)
+    c.x[:], c.w[:] = c.x.abs(), c.w.abs()
+    y = torch.full((c.n_rows, up(n_out, 8)), POISON, dtype=torch.float16, device="cuda")
+    r.grouped_matmul_device(c.layer(abi.TYPE_F16, relu), c.offsets, c.x, c.w, y)
+    # the same sums as an input gradient: samples of width n_out in the place of dx, gated by their own sign
+    gate = torch.randn(c.n_rows, up(n_out, 8), device="cuda").half()
+    wt = torch.zeros(len(sizes), n_in, up(n_out, 8), dtype=torch.float16, device="cuda")
+    wt[:, :, :n_out] = c.w.transpose(1, 2)
+    dx = torch.full_like(y, POISON)
+    p = abi.make_grouped(len(sizes), c.n_rows, n_out, n_in, abi.TYPE_F16, ld_x=up(n_out, 8), ld_w=up(n_out, 8), ld_y=c.xb.stride(0))
+    r.grouped_input_grad_device(p, c.offsets, c.x, wt, gate if relu else None, dx)
+    torch.cuda.synchronize()
+    for g, (a, b) in enumerate(c.spans):
+        exact = c.x[a:b].double() @ c.w[g].double().t()
+        bound = exact * (2.0 ** -11 + 1.001 * (512 + n_in // 512 + 1) * 2.0 ** -23)
+        assert bool(((y[a:b, :n_out].double() - exact).abs() <= bound).all()), "layer"
+        shut = ~(gate[a:b, :n_out] > 0) if relu else torch.zeros_like(exact, dtype=torch.bool)
+        assert bool((dx[a:b, :n_out][shut] == 0).all())
+        assert bool((((dx[a:b, :n_out].double() - exact).abs() <= bound) | shut).all()), "input gradient"
+    assert bool((y[:, n_out:] == POISON).all()) and bool((dx[:, n_out:] == POISON).all())
