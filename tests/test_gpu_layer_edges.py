@@ -261,3 +261,25 @@ def test_deep_sums_are_rounded_once(r, sizes, n_in, n_out, relu):  # noqa: F811
         assert bool((dx[a:b, :n_out][shut] == 0).all())
         assert bool((((dx[a:b, :n_out].double() - exact).abs() <= bound) | shut).all()), "input gradient"
     assert bool((y[:, n_out:] == POISON).all()) and bool((dx[:, n_out:] == POISON).all())
+
+
+def test_weight_grad_of_a_million_samples(r):  # noqa: F811
+    """More tiles than workers, so that a worker owns whole sums of 2048 runs.  In the 2-norm: the runs' own error (half a step
+    an instruction of 16, 32 2^-24 of a run's size) and that of adding them one by one, half a step each of a sum that grows
+    with the square root of their number: sqrt(sum of k / m for k = 1 .. m) = sqrt(m / 2) half steps."""
+    n, n_in, n_out, runs = 1 << 20, 2048, 4864, 2048
+    gen = torch.Generator(device="cuda").manual_seed(10)
+    x, dy = torch.empty(n, n_in, dtype=torch.bfloat16, device="cuda"), torch.empty(n, n_out, dtype=torch.bfloat16, device="cuda")
+    for t in (x, dy):
+        for i in range(0, n, 1 << 16):
+            t[i:i + (1 << 16)] = torch.randn(1 << 16, t.shape[1], generator=gen, device="cuda").bfloat16()
+    p = abi.make_grouped(1, n, n_in, n_out, abi.TYPE_BF16, abi.TYPE_F32)
+    space = torch.empty(r.grouped_weight_grad_workspace(p), dtype=torch.uint8, device="cuda")
+    dw = torch.full((1, n_out, n_in), POISON, device="cuda")
+    r.grouped_weight_grad_device(p, None, dy, x, dw, space)
+    torch.cuda.synchronize()
+    for cols in (slice(0, 64), slice(2500, 2564), slice(n_out - 64, n_out)):
+        exact = torch.zeros(64, n_in, dtype=torch.float64, device="cuda")
+        for i in range(0, n, 1 << 16):
+            exact += dy[i:i + (1 << 16), cols].double().t() @ x[i:i + (1 << 16)].double()
+        assert float((dw[0, cols].double() - exact).norm()) <= (32 + (runs / 2) ** 0.5) * 2.0 ** -24 * float(exact.norm())
