@@ -76,6 +76,17 @@ def _usual_offsets(t, device, count):
     return t is None or (t.dtype is _DTYPES["index"] and t.get_device() == device and t.numel() >= count and t.is_contiguous())
 
 
+def _quantize_tensors(device, type_id, rows, n_cols, values, ld_in, out, ld_out, scales, n_scales):
+    """Refuses the tensors of a quantisation; the usual ones, also values with padded rows, in one condition."""
+    d = _DTYPES or _dtypes()
+    t, n_in, n_out = d.get(type_id), (rows - 1) * (ld_in or n_cols) + n_cols, (rows - 1) * (ld_out or n_cols) + n_cols
+    if not (values.dtype is t and out.dtype is d[abi.TYPE_E4M3] and scales.dtype is d[abi.TYPE_F32]
+            and values.get_device() == out.get_device() == scales.get_device() == device
+            and out.numel() >= n_out and scales.numel() >= n_scales and out.is_contiguous() and scales.is_contiguous()
+            and (values.numel() >= n_in and values.is_contiguous() or values.stride()[-1:] == (1,) and _reach(values) >= n_in)):
+        _tensors(device, ("values", values, t, n_in), ("out", out, d[abi.TYPE_E4M3], n_out), ("scales", scales, d[abi.TYPE_F32], n_scales))
+
+
 _NEEDS = {}        # description of a layer (its bytes) -> what it needs
 
 
@@ -379,21 +390,19 @@ class Renderer:
 
     def quantize_rows_device(self, type, n_rows, n_cols, values, ld_in, out, ld_out, scales, n_rows_used=None, stream=None):
         """srf_quantize_rows: one scale per row and 128 columns; `scales` (ceil(n_cols / 128), n_rows)."""
-        d = _DTYPES or _dtypes()
-        _tensors(self.device, ("values", values, d.get(type), (n_rows - 1) * (ld_in or n_cols) + n_cols),
-                 ("out", out, d[abi.TYPE_E4M3], (n_rows - 1) * (ld_out or n_cols) + n_cols),
-                 ("scales", scales, d[abi.TYPE_F32], (n_cols + 127) // 128 * n_rows), ("n_rows_used", n_rows_used, d["index"], 1))
+        dev, n_scales = self.device, (n_cols + 127) // 128 * n_rows
+        _quantize_tensors(dev, type, n_rows, n_cols, values, ld_in, out, ld_out, scales, n_scales)
+        if not _usual_offsets(n_rows_used, dev, 1):
+            _tensors(dev, ("n_rows_used", n_rows_used, _DTYPES["index"], 1))
         self._ck(self.lib.srf_quantize_rows(self.ctx, type, n_rows, _dev_ptr(n_rows_used), n_cols, values.data_ptr(), ld_in,
-                                            out.data_ptr(), ld_out, scales.data_ptr(), _stream(self.device, stream)))
+                                            out.data_ptr(), ld_out, scales.data_ptr(), _stream(dev, stream)))
 
     def quantize_weights_device(self, type, n_matrices, n_rows, n_cols, values, ld_in, out, ld_out, scales, stream=None):
         """srf_quantize_weights: one scale per 128 x 128 block."""
-        d, rows = _DTYPES or _dtypes(), n_matrices * n_rows
-        _tensors(self.device, ("values", values, d.get(type), (rows - 1) * (ld_in or n_cols) + n_cols),
-                 ("out", out, d[abi.TYPE_E4M3], (rows - 1) * (ld_out or n_cols) + n_cols),
-                 ("scales", scales, d[abi.TYPE_F32], n_matrices * ((n_rows + 127) // 128) * ((n_cols + 127) // 128)))
+        dev, n_scales = self.device, n_matrices * ((n_rows + 127) // 128) * ((n_cols + 127) // 128)
+        _quantize_tensors(dev, type, n_matrices * n_rows, n_cols, values, ld_in, out, ld_out, scales, n_scales)
         self._ck(self.lib.srf_quantize_weights(self.ctx, type, n_matrices, n_rows, n_cols, values.data_ptr(), ld_in, out.data_ptr(),
-                                               ld_out, scales.data_ptr(), _stream(self.device, stream)))
+                                               ld_out, scales.data_ptr(), _stream(dev, stream)))
 
     def dump_samples(self, view, ray_first, ray_count, capacity):
         counts = np.zeros(ray_count, np.uint32)
