@@ -370,11 +370,12 @@ srf_status srf_grouped_weight_grad_workspace(srf_ctx* ctx, const srf_grouped_t* 
 
 /* srf_grouped_matmul on 8-bit values: y[r] = act(sum over blocks b of 128 inputs of
    d_x_scales[b][r] * d_w_scales[g][n/128][b] * (W[g] x[r])_b), with d_x_scales float[ceil(n_in/128)][n_rows] and
-   d_w_scales float[n_groups][ceil(n_out/128)][ceil(n_in/128)] as the two calls below write them. */
+   d_w_scales float[n_groups][ceil(n_out/128)][ceil(n_in/128)] as the two calls below write them.  Any fp32 scales: their
+   product may leave fp32's range where a block's term does not. */
 srf_status srf_grouped_matmul_fp8(srf_ctx* ctx, const srf_grouped_t* p, const uint64_t* d_offsets, const void* d_x,
                                   const float* d_x_scales, const void* d_w, const float* d_w_scales, void* d_y, void* stream);
 /* Samples to e4m3 with one scale per row and 128 columns: s = max |v| / 448 over the block's finite values (1 if that is 0,
-   at least 2^-126), q = the e4m3 value nearest to v / s, ties to even; infinities and NaNs become NaN.  d_in [n_rows][n_cols] of `type` (F16, BF16), d_out
+   at least 2^-126), q = the e4m3 value nearest to the fp32 quotient v / s, ties to even; infinities and NaNs become NaN.  d_in [n_rows][n_cols] of `type` (F16, BF16), d_out
    e4m3 [n_rows][n_cols], d_scales float[ceil(n_cols/128)][n_rows].  d_n_rows_used (may be NULL: all): device counter,
    rows from it on are left as they are (d_offsets + n_groups serves). */
 srf_status srf_quantize_rows(srf_ctx* ctx, int type, uint64_t n_rows, const uint64_t* d_n_rows_used, uint32_t n_cols,

@@ -26,9 +26,11 @@
 // have an error of their own that grows with sqrt(m): weight gradients have 4.8e-7 at 2^14 samples, 5.8e-7 at 2^18, 8.4e-7 at 2^20
 // where one worker owns a whole sum (shorter where the sum is cut), and some 4e-6 at 2^24.
 //
-// Measured (one B200): 32801 samples in 16 groups, 2048 -> 2043: 179 us alone (1.53 PFLOP/s, tensor pipe 93 %), 214-222 us a call
-// under the power limit (single CTAs 241); 160 samples in 64 groups, 2048 -> 1408: 63-67 us, 5.7 TB/s of matrices; 1048613
-// samples 32 -> 64: 41-43 us, 4.8 TB/s; weight gradient of 16389 x 2048 x 2048: 150 us alone and 35 for its joins.
+// Measured (several B200): 32801 samples in 16 groups, 2048 -> 2043: 178 us alone (1.54 PFLOP/s, tensor pipe 93 %), 214-224 us a
+// call under the power limit (single CTAs 241), with results in fp32 238-243; 160 samples in 64 groups, 2048 -> 1408: 63-68 us,
+// 5.4-5.9 TB/s of matrices; 1048613 samples 32 -> 64: 41-43 us, bound by the pace of the epilogue's chain (one tile of 128 x 64
+// every 1500 cycles an SM; DRAM moves 21 us' worth); weight gradient of 16389 x 2048 x 2048: 126 us alone and 27-33 for its
+// joins.
 //
 // A tile's rows behind its group's end hold the next group's samples: harmless in the first two products (an output row
 // depends on its own sample alone and those rows are not stored).  In the weight gradient they would be summed, so the
@@ -46,8 +48,8 @@ namespace {
 
 enum Mode { kLayer = 0, kInputGrad = 1, kWeightGrad = 2 };
 
-constexpr int kThreads = 384;                 // TMA, MMA, TMEM owner, spare, two sets of 4 epilogue warps (four sets: 41.2 us
-                                              // for 1048613 samples 32 -> 64 against 40.4, narrow gradients 46.9 against 44.3)
+constexpr int kThreads = 384;                 // TMA, MMA, TMEM owner, spare, two sets of 4 epilogue warps (four sets: 2 % slower
+                                              // for 1048613 samples 32 -> 64, narrow gradients 6 %)
 constexpr int kBM = 128, kBK = 64;
 constexpr uint32_t kChunk = 8;                // stages to an accumulator in LONG kernels
 constexpr uint32_t kTmemCols = 512;
@@ -82,7 +84,9 @@ template <int BN, int CG> __host__ __device__ constexpr int smem_bytes() {
 // Units of work of a group: whole output tiles for the first two products; for the weight gradient, whose work is cut evenly
 // across the CTAs (see below), the 64-sample stages of an output tile and kTileUnits in front of them, for what a tile costs
 // beside its stages: counted without, groups of few samples -- many shallow tiles -- held their CTAs up (both gradients of
-// 16389 x 2048 x 2048 in groups of 200 to 5000 samples: 324 us, with 4 units 307, 8 304, 14 302).
+// 16389 x 2048 x 2048 in groups of 200 to 5000 samples: 324 us, with 4 units 307, 8 304, 14 302).  Weight gradients alone, ragged
+// groups, units 0 / 4 / 8 / 14: 262144 x 64 x 64 in 1024 groups 80 / 74 / 74 / 74 us (in 16: 31 each), 65536 x 256 x 512 in 64
+// groups 68 / 62 / 61 / 59, 16389 x 1024 x 1024 in 100 groups 252 / 201 / 186 / 179.
 constexpr uint32_t kTileUnits = 14;
 template <int MODE, int CG>
 __device__ __forceinline__ uint32_t group_units(const Span& s, uint32_t tiles_across) {
@@ -670,7 +674,9 @@ WeightGradPlan plan_weight_grad(const srf_grouped_t& p, int sms) {
     const uint64_t busy = units < teams ? units : teams;
     // All teams together walk the samples once per tile of a group that a team works on; samples beyond what L2 holds are
     // taken in two parts (16389 x 2048 x 2048 with its input gradient: 355 us in one, 305 in two, 310 in three, 329 in
-    // four -- every part cuts as many tiles again).
+    // four -- every part cuts as many tiles again).  Weight gradients alone, in one / two parts: 131072 x 768 x 768 in 16 groups
+    // 195 / 143 us, 65536 x 1024 x 1024 in one 154 / 156, 262144 x 512 x 512 in 4 (4 tiles) 199 / 199; fewer tiles, 262144 x
+    // 256 x 256 in 16 groups, 75 / 83; fewer bytes, 4096 x 2048 x 2048 in 8, 66 / 73.
     const uint64_t bytes = p.n_rows * (p.n_in + p.n_out) * 2;
     const uint64_t parts = w.across >= 8 && bytes > (64ull << 20) ? 2 : 1;
     w.grid = (uint32_t)busy * w.cg;
@@ -710,10 +716,13 @@ uint64_t max_row_tiles(const srf_grouped_t& p, uint64_t height) {
 }
 
 TileShape pick_tile(const srf_grouped_t& p, uint32_t cols, int sms, int smallest, int cols_step) {
-    // Pairs: groups of a few 256-row tiles at least, and enough tiles for every pair.
+    // Pairs: groups of two 256-row tiles at least, and a tile for every SM.  32768 samples 1024 -> 1024 on single CTAs / pairs,
+    // even groups of 128: 123 / 125 us, 256: 84 / 81 (uneven ones waste half of a pair's last tile), 512: 73 / 64, 2048: 64 / 55;
+    // fewer tiles, 4 groups 1024 -> 256: 32 tiles 16.4 / 18.5, 128 tiles 30.7 / 28.9, 256 tiles (1024 -> 1024) 41.0 / 35.8.
     if (cols > 128 && p.n_rows / p.n_groups >= 512 && p.n_rows / 256 * ((cols + 255) / 256) >= (uint64_t)sms) return {cols_step == 32 ? (int)pair_width(cols) : 256, 2};
     // Otherwise the width that costs least: rounds of tiles over the SMs, times a tile's share of loads -- its columns, its
-    // samples, and as much as 32 columns for what every tile costs.
+    // samples, and as much as 32 columns for what every tile costs (16 to 64 choose alike; 160 samples in 64 groups, 2048 -> 1408,
+    // cold: 79.9 us, with 128 82.0; 3000 in 128, 512 -> 304: 19.7, with none 20.5, with 128 21.6).
     const uint64_t busy = p.n_groups < p.n_rows ? p.n_groups : p.n_rows;
     const uint64_t mean = (p.n_rows + busy - 1) / busy;
     const uint64_t row_tiles = mean <= 128 ? busy : p.n_rows / 128 + busy / 2;

@@ -7,13 +7,14 @@
 // (128 bytes of every row), its four instructions start a new accumulator, and two warpgroups -- each half of the tile's
 // columns -- follow one block behind.  The rest is as in srf_grouped.cu.
 //
-// Measured (one B200): 32773 samples in 8 groups, 4096 -> 2048: 300-307 us a call (1.83 PFLOP/s), 264 us alone with the
-// tensor pipe busy for 58 % of the time.  What bounds it is the accumulators' turn-over: a block's instructions take 512
+// Measured (several B200): 32773 samples in 8 groups, 4096 -> 2048: 297-307 us a call (1.8 PFLOP/s), 270 us alone with the
+// tensor pipe busy for 57 % of the time.  What bounds it is the accumulators' turn-over: a block's instructions take 512
 // cycles, reading its sums out of TMEM 455, and the two hand-overs between the issuing thread and the 16 scaling warps of a
 // pair some 700, shared by the two accumulators that TMEM holds: 835 cycles a block.  The scales themselves cost 2 %.  Narrower
 // tiles with more accumulators or more warps were slower (192 columns and three sets of warps 333 us, 128 columns and four
-// accumulators 370), as were single CTAs (330 us alone).  Few samples are bound by the matrices: 131 samples in 32 groups of
-// 2048 x 2048, 135 MB, 31-33 us (floor 20.6; 1.73 tiles an SM).
+// accumulators 370), as were single CTAs (330 us alone).  Few samples: 131 samples in 32 groups of 2048 x 2048, 135 MB, 31-33
+// us (floor 20.6): whole tiles only, 1.73 an SM round up to 2, which makes 23.8 of them; the rest is start-up and the hand-over
+// of every block.
 #include <cstring>
 #include "srf_layers.cuh"
 #include "srf_tile.cuh"

@@ -2,7 +2,7 @@
 //
 // A block shares one scale s = amax / 448, amax over the block's finite values (1 where that is 0, and at least 2^-126,
 // below which a quotient could leave the range); q = the e4m3 value nearest to v / s, ties to even.  Infinities and
-// NaNs become e4m3's NaN and do not touch the block's other values.
+// NaNs become e4m3's NaN and do not touch the block's other values.  v / s is the fp32 quotient.
 //
 // v / s must be the correctly rounded quotient: one step off moves values that lie next to a tie.  With r the correctly
 // rounded 1 / s and q0 = v r, q0 + r (v - q0 s) -- two fused operations -- is that quotient (Markstein, IBM J. Res. Dev. 34,
@@ -13,7 +13,7 @@
 // maximum is not finite is gone through again, value by value.
 //
 // Bound by memory: two bytes read, one written per value, one pass (the block stays in registers between the maximum
-// and the quotients).  65539 x 2048: 70 us alone, 74-78 a call, 5.3 TB/s; 66 % of the issue slots are taken.
+// and the quotients).  65539 x 2048: 71 us alone, 75-78 a call, 5.2-5.4 TB/s; 66 % of the issue slots are taken.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "srf_layers.cuh"
@@ -167,7 +167,7 @@ k_quantize_rows(int bf16, uint64_t n_rows, const uint64_t* __restrict__ n_used, 
         for (int i = 0; i < kRowsPerWarp; ++i) v[i] = row0 + i < rows ? load8(in + i * ld_in + col, have) : make_uint4(0u, 0u, 0u, 0u);
     }
     // Every lane makes the scale of one of its half's four blocks -- the two divisions of a scale cost as much as all the rest
-    // of a block, and 16 lanes repeating them for every row made the kernel issue-bound (65539 x 2048: 88 us, 82 without it).
+    // of a block, and 16 lanes repeating them for every row made the kernel issue-bound (7 % of 65539 x 2048's time).
     uint32_t mine = 0;
     bool finite_all = true;
 #pragma unroll

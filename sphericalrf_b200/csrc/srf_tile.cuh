@@ -479,7 +479,8 @@ __device__ __forceinline__ void fma2(uint64_t& sum, uint64_t a, uint64_t b) {
 __device__ __forceinline__ void add2(uint64_t& sum, uint64_t a) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum) : "l"(a)); }
 
 // Registers of kernels whose 8 epilogue warps hold 128 sums a thread beside two pieces of 32 in flight.  A block of 384 is
-// launched with 168 a thread (64512).
+// launched with 168 a thread (64512); a share of 72 for the issuing warps would use them all.  The compiler keeps to 168 for the
+// whole kernel and spills 90 to 130 bytes in the 256-column kernels with such sums, 100 in the 8-bit ones, with either share.
 constexpr int kRegsIssue = 64, kRegsSum = 216;
 static_assert(128 * kRegsIssue + 256 * kRegsSum <= 384 * 168, "a larger share would wait for registers forever");
 __device__ __forceinline__ void regs_for_issue() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsIssue)); }
