@@ -283,3 +283,49 @@ def test_weight_grad_of_a_million_samples(r):  # noqa: F811
         for i in range(0, n, 1 << 16):
             exact += dy[i:i + (1 << 16), cols].double().t() @ x[i:i + (1 << 16)].double()
         assert float((dw[0, cols].double() - exact).norm()) <= (32 + (runs / 2) ** 0.5) * 2.0 ** -24 * float(exact.norm())
+
+
+def test_8_bit_chains_captured_on_two_streams(r):  # noqa: F811
+    """Quantisation and two 8-bit layers, captured once and replayed on two streams at a time, on new samples: eager bits."""
+    def make(seed, counts):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        n, k = sum(counts), 256
+        s = dict(n=n, k=k, off=torch.from_numpy(np.concatenate([[0], np.cumsum(counts)])).cuda(), groups=len(counts))
+        s["h"] = torch.randn(n, k, generator=gen, device="cuda").bfloat16()
+        s["w"] = (torch.randn(len(counts), k, k, generator=gen, device="cuda") / 16).bfloat16()
+        s["q"], s["qs"] = torch.zeros(n, k, dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros(2, n, device="cuda")
+        s["w8"], s["ws"] = torch.zeros(len(counts), k, k, dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros(len(counts), 2, 2, device="cuda")
+        s["y"] = torch.zeros(2, n, k, dtype=torch.bfloat16, device="cuda")
+        return s
+
+    def step(s):
+        layer = abi.make_grouped(s["groups"], s["n"], s["k"], s["k"], abi.TYPE_E4M3, abi.TYPE_BF16, abi.ACT_RELU)
+        r.quantize_weights_device(abi.TYPE_BF16, s["groups"], s["k"], s["k"], s["w"], s["k"], s["w8"], s["k"], s["ws"])
+        for x, y in ((s["h"], s["y"][0]), (s["y"][0], s["y"][1])):
+            r.quantize_rows_device(abi.TYPE_BF16, s["n"], s["k"], x, s["k"], s["q"], s["k"], s["qs"], n_rows_used=s["off"][-1:])
+            r.grouped_matmul_fp8_device(layer, s["off"], s["q"], s["qs"], s["w8"], s["ws"], y)
+
+    chains, graphs = [make(1, [700, 0, 33, 5000]), make(2, [1, 128, 2000])], []
+    for s in chains:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step(s)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in chains]
+    for turn in range(3):
+        for s in chains:
+            s["h"].mul_(0.5 + turn).neg_()
+            s["y"].zero_()
+        torch.cuda.synchronize()
+        for _ in range(2):
+            for g, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+        torch.cuda.synchronize()
+        got = [s["y"].clone() for s in chains]
+        for s, y in zip(chains, got):
+            s["y"].zero_()
+            step(s)
+            torch.cuda.synchronize()
+            assert torch.equal(s["y"], y) and bool((y != 0).any())
+    r.check_errors()
